@@ -24,6 +24,9 @@ enum EpiKind : int {
   EPI_I8_F32 = 7,      // int8 product: f32 out = acc * mod[row] * norm_q[col] (a measured experiment)
 };
 
+// STATUS_BAD_ARG of exn_device.cuh, for host code: what a kernel read from the device was out of range
+constexpr int STATUS_BAD_ARG_BIT = 4;
+
 // ranks of a sequence-parallel group that kernels address directly (peer pointers)
 constexpr int kMaxSp = 16;
 
@@ -134,6 +137,57 @@ int attention_launch(const AttnArgs& a, int* d_status, cudaStream_t st);
 int attention_prepare();
 int gemm_prepare();
 int gemm_q8_prepare();
+
+// Causal attention of packed sequences (attn_packed.cu), head dim 128, bf16 or (F16) fp16: sequence s
+// owns query rows q_offsets[s] .. q_offsets[s + 1] - 1 of ROWS and key rows kv_offsets[s] .. of KV_ROWS
+// or, with KV_LENS, the KV_LENS[s] rows from s * KV_STRIDE on; its queries are its last positions.
+// Row strides in elements, multiples of 8; bases 16-byte aligned; offsets and lengths on the device.
+// 0, -1 (too many tiles), -4 (tensor map) or a cudaError_t.
+struct PackedArgs {
+  int f16 = 0, heads = 0, kv_heads = 0, nseq = 0;
+  const int* q_offsets = nullptr;
+  const int* kv_offsets = nullptr;
+  const int* kv_lens = nullptr;
+  long long kv_stride = 0, rows = 0, kv_rows = 0;
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  void* out = nullptr;
+  long long ld_q = 0, ld_k = 0, ld_v = 0, ld_out = 0;
+  float scale_log2 = 0.f;
+};
+int packed_launch(const PackedArgs& a, int* d_status, cudaStream_t st);
+int packed_prepare();
+
+// The 8-bit key/value cache (attn_cache.cu): exn_kv_cache of include/exn_b200.h
+constexpr int kPage = 64;  // tokens a page
+struct CacheArgs {
+  int kv_heads = 0, nseq = 0, pages = 0, table_ld = 0;
+  int8_t *k = nullptr, *v = nullptr;               // codes [pages][kv_heads][64][128]
+  float *k_scale = nullptr, *v_scale = nullptr;    // [pages][kv_heads], powers of two
+  const int* table = nullptr;                      // [nseq][table_ld]: page of positions 64 i .. 64 i + 63
+  const int* lens = nullptr;                       // [nseq]: positions held, the call's rows among them
+};
+// rows offsets[s] .. offsets[s + 1] - 1 of K and V (row strides in elements) are sequence s's last positions
+int cache_write_launch(const CacheArgs& c, int f16, const int* offsets, long long rows, const void* k, long long ld_k,
+                       const void* v, long long ld_v, int* d_status, cudaStream_t st);
+int cache_read_launch(const CacheArgs& c, int f16, const int* offsets, long long rows, void* k, long long ld_k,
+                      void* v, long long ld_v, int* d_status, cudaStream_t st);
+// every position of every sequence: position j of sequence s to row s * table_ld * 64 + j of K and V
+// [nseq * table_ld * 64][kv_heads * 128]
+int cache_dense_launch(const CacheArgs& c, int f16, void* k, void* v, int* d_status, cudaStream_t st);
+struct CacheAttnArgs {
+  CacheArgs c;
+  int f16 = 0, heads = 0;
+  const int* offsets = nullptr;
+  long long rows = 0;
+  const void* q = nullptr;
+  long long ld_q = 0;
+  void* out = nullptr;
+  long long ld_out = 0;
+  float scale_log2 = 0.f;
+};
+// few rows a sequence: one pass over the codes on CUDA's warp-level MMA, the keys split over clusters
+int cache_attend_launch(const CacheAttnArgs& a, int sms, int* d_status, cudaStream_t st);
+int cache_prepare();
 
 // C = A . (q d)^T with the weights as Q8_0 (gemm_q8.cu): QS int8 [N][K], DK the fp16 scales laid out
 // by k-block ([K/64][N][2], q8_scales_by_kblock_launch from GGUF's [N][K/32]).  Epilogues EPI_F32

@@ -53,6 +53,16 @@ class EncConfig(ctypes.Structure):
                 ("ffn", ctypes.c_int), ("vocab", ctypes.c_int), ("theta", ctypes.c_double), ("device", ctypes.c_int)]
 
 
+class KvCache(ctypes.Structure):
+    """exn_kv_cache: keys and values in 8 bits on the device, in memory that the caller keeps (pointers as
+    ints, e.g. torch tensors' data_ptr()).  K, V: int8 codes [pages][kv_heads][64][128]; K_SCALE, V_SCALE:
+    float32 [pages][kv_heads]; TABLE: int32 [nseq][table_ld]; LENS: int32 [nseq]."""
+    _fields_ = [("kv_heads", ctypes.c_int), ("nseq", ctypes.c_int), ("pages", ctypes.c_int),
+                ("table_ld", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("lens", ctypes.c_void_p)]
+
+
 class Ref(ctypes.Structure):
     _fields_ = [("a", ctypes.c_int), ("latent", ctypes.POINTER(ctypes.c_float)), ("rh", ctypes.c_int),
                 ("rw", ctypes.c_int)]
@@ -72,6 +82,7 @@ def lib():
     H = ctypes.c_void_p
     fp = ctypes.POINTER(ctypes.c_float)
     vp = ctypes.c_void_p
+    i64 = ctypes.c_int64
     sigs = {
         "exn_abi_version": (ctypes.c_int, []),
         "exn_default_config": (None, [ctypes.POINTER(Config)]),
@@ -117,6 +128,20 @@ def lib():
         "exn_enc_release": (ctypes.c_int, [H]),
         "exn_test_enc_last_ms": (ctypes.c_int, [H, ctypes.POINTER(ctypes.c_double)]),
         "exn_test_enc_weights_digest": (ctypes.c_int, [H, ctypes.POINTER(ctypes.c_uint64)]),
+        "exn_attn_open": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(H)]),
+        "exn_attn_close": (None, [H]),
+        "exn_attn_last_error": (ctypes.c_char_p, [H]),
+        "exn_attn_sync": (ctypes.c_int, [H, vp]),
+        "exn_attn_packed": (ctypes.c_int, [H] + [ctypes.c_int] * 4 + [vp] * 2 + [i64] * 2 + [vp, i64] * 4 +
+                            [ctypes.c_double, vp]),
+        "exn_attn_cache_write": (ctypes.c_int, [H, ctypes.POINTER(KvCache), ctypes.c_int, vp, i64] + [vp, i64] * 2 +
+                                 [vp]),
+        "exn_attn_cache_read": (ctypes.c_int, [H, ctypes.POINTER(KvCache), ctypes.c_int, vp, i64] + [vp, i64] * 2 +
+                                [vp]),
+        "exn_attn_cache_attend": (ctypes.c_int, [H, ctypes.POINTER(KvCache), ctypes.c_int, ctypes.c_int, vp, i64] +
+                                  [vp, i64] * 2 + [ctypes.c_double, vp, ctypes.c_size_t, vp]),
+        "exn_attn_cache_workspace": (ctypes.c_int, [H, ctypes.POINTER(KvCache), ctypes.c_int, i64,
+                                                    ctypes.POINTER(ctypes.c_size_t)]),
         "exn_release": (ctypes.c_int, [H]),
         "exn_comm_unique_id": (ctypes.c_int, [vp]),
         "exn_comm_init": (ctypes.c_int, [H, vp, ctypes.c_int, ctypes.c_int]),
@@ -484,6 +509,73 @@ class Encoder:
         d = ctypes.c_uint64()
         self._ck(lib().exn_test_enc_weights_digest(self.h, ctypes.byref(d)))
         return d.value
+
+
+class Attention:
+    """The attention operators of include/exn_b200.h on one CUDA device.  Every pointer is an int (a device
+    address, e.g. a torch tensor's data_ptr()); row strides count elements, 0 for contiguous rows; STREAM is
+    an int cudaStream_t, 0 CUDA's default stream.  The calls queue their kernels and return."""
+
+    def __init__(self, device=0):
+        h = ctypes.c_void_p()
+        rc = lib().exn_attn_open(device, ctypes.byref(h))
+        if rc != EXN_OK:
+            raise ExnError(rc, lib().exn_attn_last_error(None).decode(errors="replace"))
+        self.h = h
+        self.L = lib()
+
+    def _ck(self, rc):
+        if rc != EXN_OK:
+            raise ExnError(rc, lib().exn_attn_last_error(self.h).decode(errors="replace"))
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().exn_attn_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+    def packed(self, q, k, v, out, offsets, nseq, rows, heads, kv_heads, dtype=GGML_BF16, ld_q=0, ld_k=0, ld_v=0,
+               ld_out=0, kv_offsets=None, kv_rows=None, scale=0.0, stream=0):
+        """Causal attention of NSEQ packed sequences; KV_OFFSETS and KV_ROWS where the keys' rows are not the
+        queries'."""
+        self._ck(self.L.exn_attn_packed(self.h, dtype, heads, kv_heads, nseq, offsets, kv_offsets, rows,
+                                        rows if kv_rows is None else kv_rows, q, ld_q, k, ld_k, v, ld_v, out, ld_out,
+                                        scale, stream))
+
+    def cache_write(self, cache, k, v, offsets, rows, dtype=GGML_BF16, ld_k=0, ld_v=0, stream=0):
+        """New keys and values, the last positions of their sequences, into CACHE (a KvCache)."""
+        self._ck(self.L.exn_attn_cache_write(self.h, cache, dtype, offsets, rows, k, ld_k, v, ld_v, stream))
+
+    def cache_read(self, cache, k, v, offsets, rows, dtype=GGML_BF16, ld_k=0, ld_v=0, stream=0):
+        """The sequences' last positions out of CACHE."""
+        self._ck(self.L.exn_attn_cache_read(self.h, cache, dtype, offsets, rows, k, ld_k, v, ld_v, stream))
+
+    def cache_workspace(self, cache, rows, heads):
+        """Bytes that cache_attend needs for ROWS rows."""
+        n = ctypes.c_size_t()
+        self._ck(self.L.exn_attn_cache_workspace(self.h, cache, heads, rows, ctypes.byref(n)))
+        return n.value
+
+    def cache_attend(self, cache, q, out, offsets, rows, heads, dtype=GGML_BF16, ld_q=0, ld_out=0, scale=0.0,
+                     workspace=None, workspace_bytes=0, stream=0):
+        """Attention of the sequences' last positions over CACHE."""
+        self._ck(self.L.exn_attn_cache_attend(self.h, cache, dtype, heads, offsets, rows, q, ld_q, out, ld_out, scale,
+                                              workspace, workspace_bytes, stream))
+
+    def sync(self, stream=0):
+        """Wait for STREAM; raises what the kernels found wrong since the last sync."""
+        self._ck(self.L.exn_attn_sync(self.h, stream))
 
 
 # ---- the reference's names

@@ -244,6 +244,82 @@ int exn_enc_states_device(exn_enc* e, const int32_t* ids, int n, const int32_t* 
 /* The encoder's scratch freed (the weights stay). */
 int exn_enc_release(exn_enc* e);
 
+/* ---- Attention on device memory: the language model's operators that the prompt encoder is made of,
+ * for programs that keep their own activations or caches on the GPU.  No counterpart in the reference,
+ * which encodes one prompt a call and keeps nothing (src/encoder.lisp:143-183).
+ *
+ * Head dimension 128.  TYPE is EXN_GGML_BF16 or EXN_GGML_F16, the type of q, k, v and the outputs; sums,
+ * maxima and the softmax are fp32.  Query head h reads key/value head h / (heads / kv_heads), heads a
+ * multiple of kv_heads and at most 128 times it.  Every pointer but the handle's and *CACHE itself is
+ * device memory of the handle's device.  Rows are packed: row r of a matrix starts at r * ld elements,
+ * its heads side by side; ld a multiple of 8 (0: the rows are contiguous), bases 16-byte aligned.
+ * OFFSETS (int32, nseq + 1, on the device, not decreasing, from 0) says which rows are whose: sequence
+ * s has rows OFFSETS[s] .. OFFSETS[s + 1] - 1, possibly none; rows from OFFSETS[nseq] on, up to ROWS,
+ * are left as they are.  SCALE multiplies the scores (0: 1 / sqrt(128)).
+ *
+ * The calls check what the host can see and queue kernels on STREAM (a cudaStream_t of the device; NULL
+ * is CUDA's default stream): no allocation, no host wait, capturable into a CUDA graph, the current
+ * device left as it was.  Lengths and tables are read when the kernels run.  What the kernels find wrong
+ * there (offsets that decrease or pass ROWS, lengths shorter than a sequence's rows, a page that is not
+ * the pool's) they leave out, and exn_attn_sync reports it.  The calls keep nothing between them, so
+ * calls on different streams may run at once, except on the same workspace or, where one writes, on the
+ * same pages. */
+typedef struct exn_attn exn_attn;
+
+int exn_attn_open(int device, exn_attn** out);
+void exn_attn_close(exn_attn* a);
+const char* exn_attn_last_error(const exn_attn* a);
+
+/* Wait for STREAM and report what the kernels of this handle found wrong since the last such call:
+ * EXN_EINVAL for bad offsets, lengths or pages, EXN_ETIMEOUT for a kernel that gave up. */
+int exn_attn_sync(exn_attn* a, void* stream);
+
+/* Causal attention of NSEQ packed sequences: q and out ROWS x heads * 128, k and v KV_ROWS x kv_heads *
+ * 128.  KV_OFFSETS gives the key rows of each sequence (NULL: Q's offsets); a sequence's queries are its
+ * last positions: of nq query and nk key rows, query row i sees keys 0 .. i + nk - nq.  A row that sees
+ * no key is 0.  An infinity or a NaN reaches only the rows that see it. */
+int exn_attn_packed(exn_attn* a, int type, int heads, int kv_heads, int nseq, const int32_t* q_offsets,
+                    const int32_t* kv_offsets, int64_t rows, int64_t kv_rows, const void* q, int64_t ld_q,
+                    const void* k, int64_t ld_k, const void* v, int64_t ld_v, void* out, int64_t ld_out,
+                    double scale, void* stream);
+
+/* Keys and values held in 8 bits, in pages of 64 positions.  A page has, for every key/value head, codes
+ * int8 [64][128] and one scale, a power of two: the smallest >= 2^-126 with max |x| <= 127 scale over
+ * what the page has held since its first position was last written; a value is code * scale, off by at
+ * most scale / 2 when it is written and, after later tokens made the scale grow, by less than the scale.
+ * A page that is given an infinity or a NaN takes the scale NaN, and rows that see a position of it are
+ * NaN, until its first position is written anew. */
+typedef struct exn_kv_cache {
+  int kv_heads;
+  int nseq;
+  int pages;             /* the pool's */
+  int table_ld;          /* entries of a table row: a sequence has at most 64 * table_ld positions */
+  int8_t* k;             /* codes [pages][kv_heads][64][128], 16-byte aligned, and v */
+  int8_t* v;
+  float* k_scale;        /* [pages][kv_heads] */
+  float* v_scale;
+  const int32_t* table;  /* [nseq][table_ld]: the page of positions 64 i .. 64 i + 63; entries behind a
+                          * sequence's last page are not read */
+  const int32_t* lens;   /* [nseq]: positions a sequence holds, those of the call's rows among them */
+} exn_kv_cache;
+
+/* New keys and values into the cache: the rows of sequence s are its last positions, lens[s] - count ..
+ * lens[s] - 1.  Pages that two sequences share must not be written. */
+int exn_attn_cache_write(exn_attn* a, const exn_kv_cache* cache, int type, const int32_t* offsets, int64_t rows,
+                         const void* k, int64_t ld_k, const void* v, int64_t ld_v, void* stream);
+
+/* The last count positions of every sequence out of the cache (all of them when count = lens[s]). */
+int exn_attn_cache_read(exn_attn* a, const exn_kv_cache* cache, int type, const int32_t* offsets, int64_t rows,
+                        void* k, int64_t ld_k, void* v, int64_t ld_v, void* stream);
+
+/* Attention over the cache: the rows of sequence s, its last positions, each see the positions up to
+ * their own (their keys and values written before).  WORKSPACE: exn_attn_cache_workspace's bytes for these
+ * ROWS and heads, 256-byte aligned, not shared by calls that may run at once (NULL when 0 bytes). */
+int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int heads, const int32_t* offsets,
+                          int64_t rows, const void* q, int64_t ld_q, void* out, int64_t ld_out, double scale,
+                          void* workspace, size_t workspace_bytes, void* stream);
+int exn_attn_cache_workspace(exn_attn* a, const exn_kv_cache* cache, int heads, int64_t rows, size_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif
