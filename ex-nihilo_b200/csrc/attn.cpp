@@ -130,17 +130,6 @@ int launched(exn_attn* a, const char* fn, int r) {
   return afail(a, EXN_ECUDA, "%s: launch failed: %s", fn, cudaGetErrorString(static_cast<cudaError_t>(r)));
 }
 
-// Rows (tokens times the query heads of a key/value head) a sequence, on average, from which the cache
-// is turned into 16 bits once and read by the packed kernel's tensor-core tiles; below, the codes are
-// read directly, 16 rows at a time.
-constexpr int64_t kDenseRows = 64;
-
-bool dense_path(const exn_kv_cache* c, int heads, int64_t rows) {
-  return rows * (heads / c->kv_heads) > kDenseRows * c->nseq;
-}
-
-int64_t dense_rows(const exn_kv_cache* c) { return static_cast<int64_t>(c->nseq) * c->table_ld * kPage; }
-
 }  // namespace
 
 extern "C" {
@@ -297,7 +286,7 @@ int exn_attn_cache_workspace(exn_attn* a, const exn_kv_cache* cache, int heads, 
   CacheArgs c;
   if ((rc = check_cache(a, fn, cache, &c)) || (rc = check_heads(a, fn, heads, c.kv_heads))) return rc;
   if (!bytes || rows < 0 || rows > kMaxRows) return afail(a, EXN_EINVAL, "%s: null result, or %lld rows", fn, static_cast<long long>(rows));
-  *bytes = dense_path(cache, heads, rows) ? static_cast<size_t>(dense_rows(cache)) * c.kv_heads * 128 * 2 * 2 : 0;
+  *bytes = c.nseq ? cache_attention_workspace(c, heads, rows) : 0;
   return EXN_OK;
 }
 
@@ -316,39 +305,12 @@ int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int 
   if ((rc = check_matrix(a, fn, "q", q, &ld_q, heads)) || (rc = check_matrix(a, fn, "out", out, &ld_out, heads)))
     return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool dense = dense_path(cache, heads, rows);
-  const int64_t drows = dense_rows(cache);
-  const size_t need = dense ? static_cast<size_t>(drows) * p.c.kv_heads * 128 * 2 * 2 : 0;
+  const size_t need = cache_attention_workspace(p.c, heads, rows);
   if (need > workspace_bytes || (need && !workspace))
     return afail(a, EXN_EINVAL, "%s: a workspace of %zu bytes, %zu needed", fn, workspace ? workspace_bytes : 0, need);
   if (need && !aligned(workspace, 256)) return afail(a, EXN_EINVAL, "%s: the workspace is not 256-byte aligned", fn);
-  if (dense && drows > kMaxRows) return afail(a, EXN_EINVAL, "%s: room for %lld positions", fn, static_cast<long long>(drows));
   OnDevice on(a->device);
   ACK(on.rc);
-  if (dense) {
-    uint16_t* k = static_cast<uint16_t*>(workspace);
-    uint16_t* v = k + static_cast<size_t>(drows) * p.c.kv_heads * 128;
-    if ((rc = launched(a, fn, cache_dense_launch(p.c, type == EXN_GGML_F16, k, v, a->d_status, st)))) return rc;
-    PackedArgs d;
-    d.f16 = type == EXN_GGML_F16;
-    d.heads = heads;
-    d.kv_heads = p.c.kv_heads;
-    d.nseq = p.c.nseq;
-    d.q_offsets = offsets;
-    d.kv_lens = p.c.lens;
-    d.kv_stride = static_cast<int64_t>(p.c.table_ld) * kPage;
-    d.rows = rows;
-    d.kv_rows = drows;
-    d.q = q;
-    d.k = k;
-    d.v = v;
-    d.out = out;
-    d.ld_q = ld_q;
-    d.ld_k = d.ld_v = static_cast<int64_t>(p.c.kv_heads) * 128;
-    d.ld_out = ld_out;
-    d.scale_log2 = p.scale_log2;
-    return launched(a, fn, packed_launch(d, a->d_status, st));
-  }
   p.f16 = type == EXN_GGML_F16;
   p.heads = heads;
   p.offsets = offsets;
@@ -357,7 +319,7 @@ int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int 
   p.ld_q = ld_q;
   p.out = out;
   p.ld_out = ld_out;
-  return launched(a, fn, cache_attend_launch(p, a->sms, a->d_status, st));
+  return launched(a, fn, cache_attention(p, workspace, workspace_bytes, a->sms, a->d_status, st));
 }
 
 }  // extern "C"

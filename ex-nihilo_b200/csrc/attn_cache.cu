@@ -763,7 +763,7 @@ int cache_read_launch(const CacheArgs& c, int f16, const int* offsets, long long
                                      static_cast<uint16_t*>(k), ld_k, static_cast<uint16_t*>(v), ld_v, d_status));
 }
 
-int cache_dense_launch(const CacheArgs& c, int f16, void* k, void* v, int* d_status, cudaStream_t st) {
+static int dense_launch(const CacheArgs& c, int f16, void* k, void* v, int* d_status, cudaStream_t st) {
   const long long blocks = static_cast<long long>(c.nseq) * c.table_ld * c.kv_heads;
   if (blocks > 0x7fffffffll) return -1;
   const long long ld = static_cast<long long>(c.kv_heads) * 128;
@@ -780,7 +780,21 @@ int cache_prepare() {
   return static_cast<int>(e);
 }
 
-int cache_attend_launch(const CacheAttnArgs& a, int sms, int* d_status, cudaStream_t st) {
+// Rows (tokens times the query heads of a key/value head) a sequence, on average, beyond which the cache
+// is turned into 16 bits once and read by the packed kernel's tensor-core tiles; up to it, the codes are
+// read directly, 16 rows at a time.
+constexpr long long kDenseRows = 64;
+
+static bool dense_path(const CacheArgs& c, int heads, long long rows) {
+  return rows * (heads / c.kv_heads) > kDenseRows * c.nseq;
+}
+static long long dense_rows(const CacheArgs& c) { return static_cast<long long>(c.nseq) * c.table_ld * kPage; }
+
+size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows) {
+  return dense_path(c, heads, rows) ? static_cast<size_t>(dense_rows(c)) * c.kv_heads * 128 * 2 * 2 : 0;
+}
+
+static int attend_launch(const CacheAttnArgs& a, int sms, int* d_status, cudaStream_t st) {
   const CacheArgs& c = a.c;
   const int g = a.heads / c.kv_heads;
   CUtensorMap tk, tv;
@@ -809,6 +823,35 @@ int cache_attend_launch(const CacheAttnArgs& a, int sms, int* d_status, cudaStre
     e = nt == 1 ? launch_attend<false, 4, 1>(a, tk, tv, items, ncta, hpt, head_tiles, tpt, d_status, st)
                 : launch_attend<false, 4, 2>(a, tk, tv, items, ncta, hpt, head_tiles, tpt, d_status, st);
   return static_cast<int>(e);
+}
+
+int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, int* d_status, cudaStream_t st) {
+  const CacheArgs& c = a.c;
+  if (!dense_path(c, a.heads, a.rows)) return attend_launch(a, sms, d_status, st);
+  if (ws_bytes < cache_attention_workspace(c, a.heads, a.rows) || dense_rows(c) > 0x7fffffffll) return -1;
+  uint16_t* k = static_cast<uint16_t*>(ws);
+  uint16_t* v = k + static_cast<size_t>(dense_rows(c)) * c.kv_heads * 128;
+  const int r = dense_launch(c, a.f16, k, v, d_status, st);
+  if (r) return r;
+  PackedArgs p;
+  p.f16 = a.f16;
+  p.heads = a.heads;
+  p.kv_heads = c.kv_heads;
+  p.nseq = c.nseq;
+  p.q_offsets = a.offsets;
+  p.kv_lens = c.lens;
+  p.kv_stride = static_cast<long long>(c.table_ld) * kPage;
+  p.rows = a.rows;
+  p.kv_rows = dense_rows(c);
+  p.q = a.q;
+  p.k = k;
+  p.v = v;
+  p.out = a.out;
+  p.ld_q = a.ld_q;
+  p.ld_k = p.ld_v = static_cast<long long>(c.kv_heads) * 128;
+  p.ld_out = a.ld_out;
+  p.scale_log2 = a.scale_log2;
+  return packed_launch(p, d_status, st);
 }
 
 }  // namespace exn

@@ -11,7 +11,9 @@
 //     (EPI_QKV), the residual add (EPI_GATE_RESID with a gate of ones), SwiGLU
 //     (EPI_SWIGLU over gate and up rows interleaved by 128);
 //   * attention is the DiT's tcgen05 kernel with every row causal and query
-//     head i reading key/value head i / 4;
+//     head i reading key/value head i / 4; several prompts in one pass
+//     (exn_enc_states_packed) take the packed kernel, and prompts continued
+//     from kept keys and values (exn_enc_extend) the 8-bit cache's kernels;
 //   * the residual stream and the embedding table are fp32; the embedding rows
 //     are the file's values exactly.
 #include <cuda_runtime.h>
@@ -21,7 +23,9 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <map>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -87,8 +91,24 @@ struct exn_enc {
   // scratch for up to cap tokens
   int cap = 0;
   void* scratch = nullptr;
+  // offsets and lengths of a pass of several sequences, and the cached attention's workspace
+  int* seqs = nullptr;
+  size_t seqs_cap = 0;
+  void* attn_ws = nullptr;
+  size_t attn_ws_cap = 0;
   cudaEvent_t ev[2] = {nullptr, nullptr};
   double last_ms = 0;
+};
+
+// Kept keys and values of nseq sequences, every block's: the 8-bit cache of attn_cache.cu with a pool of
+// pages a block, sequence s's the pages s * ld .. s * ld + ld - 1
+struct exn_enc_cache {
+  exn_enc* owner = nullptr;
+  int device = 0, nseq = 0, ld = 0, layers = 0, kv_heads = 0;
+  int8_t* codes = nullptr;  // [layer][k, v][pages][kv_heads][64][128]
+  float* scales = nullptr;  // [layer][k, v][pages][kv_heads]
+  int* table = nullptr;
+  std::vector<int> lens;
 };
 
 namespace {
@@ -327,12 +347,79 @@ int gemm_split(exn_enc* e, const bf16* a, const bf16* b, int n, int N, int K, in
   return gemm(e, g, what, layer);
 }
 
+// How the rows of a pass are several sequences': their offsets on the device and, for a pass that
+// continues them, the cache with its lengths (this pass's rows among them) on the device
+struct Pass {
+  int nseq = 0;
+  const int* offsets = nullptr;
+  const exn_enc_cache* cache = nullptr;
+  const int* lens = nullptr;
+  void* ws = nullptr;
+  size_t ws_bytes = 0;
+};
+
+// block LI's part of a cache
+CacheArgs cache_args(const exn_enc_cache* c, int li, const int* lens) {
+  CacheArgs a;
+  a.kv_heads = c->kv_heads;
+  a.nseq = c->nseq;
+  a.pages = c->nseq * c->ld;
+  a.table_ld = c->ld;
+  const size_t heads = static_cast<size_t>(a.pages) * c->kv_heads, bytes = heads * kPage * kHeadDim;
+  a.k = c->codes + 2 * li * bytes;
+  a.v = a.k + bytes;
+  a.k_scale = c->scales + 2 * li * heads;
+  a.v_scale = a.k_scale + heads;
+  a.table = c->table;
+  a.lens = lens;
+  return a;
+}
+
+// attention of a pass of several sequences: s.q, s.k, s.v -> s.xn
+int attend_sequences(exn_enc* e, int li, int n, const Scratch& s, const Pass& ps) {
+  const exn_enc_config& c = e->cfg;
+  const int q = q_width(c), kv = kv_width(c);
+  const float scale_log2 = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(kHeadDim)));
+  int r;
+  if (!ps.cache) {
+    PackedArgs a;
+    a.heads = c.heads;
+    a.kv_heads = c.kv_heads;
+    a.nseq = ps.nseq;
+    a.q_offsets = a.kv_offsets = ps.offsets;
+    a.rows = a.kv_rows = n;
+    a.q = s.q;
+    a.k = s.k;
+    a.v = s.v;
+    a.out = s.xn;
+    a.ld_q = a.ld_out = q;
+    a.ld_k = a.ld_v = kv;
+    a.scale_log2 = scale_log2;
+    r = packed_launch(a, e->d_status, e->st);
+  } else {
+    CacheAttnArgs a;
+    a.c = cache_args(ps.cache, li, ps.lens);
+    a.heads = c.heads;
+    a.offsets = ps.offsets;
+    a.rows = n;
+    a.q = s.q;
+    a.ld_q = a.ld_out = q;
+    a.out = s.xn;
+    a.scale_log2 = scale_log2;
+    r = cache_write_launch(a.c, 0, ps.offsets, n, s.k, kv, s.v, kv, e->d_status, e->st);
+    if (!r) r = cache_attention(a, ps.ws, ps.ws_bytes, e->sms, e->d_status, e->st);
+  }
+  if (r) return efail(e, EXN_ECUDA, "encoder block %d: attention (%d rows, %d sequences) launch failed: %d", li, n, ps.nseq, r);
+  return EXN_OK;
+}
+
 // one block of the text model over the N rows of S (x updated in place).  A thin prompt's GEMMs
 // run split along K into fp32 partials, summed (in split order) by the kernel that applies the
 // epilogue; a longer prompt's have the epilogue fused.  After a split residual GEMM the summing
 // kernel also writes the next RMS norm's output.  *NORMED: on entry, whether s.xn already holds
-// this block's attn_norm output; on return, whether it holds the next block's.
-int block(exn_enc* e, int li, int n, const Scratch& s, bool* normed) {
+// this block's attn_norm output; on return, whether it holds the next block's.  PS: the rows are several
+// sequences' (null: one prompt's).
+int block(exn_enc* e, int li, int n, const Scratch& s, bool* normed, const Pass* ps) {
   const exn_enc_config& c = e->cfg;
   const EncLayer& L = e->layers[li];
   const float* next_norm = li + 1 < c.layers ? e->layers[li + 1].attn_norm : nullptr;
@@ -365,7 +452,9 @@ int block(exn_enc* e, int li, int n, const Scratch& s, bool* normed) {
     g.ep.v = s.v;
     if ((rc = gemm(e, g, "q/k/v", li))) return rc;
   }
-  {  // causal attention, query head i on key/value head i / (heads / kv_heads)
+  if (ps) {
+    if ((rc = attend_sequences(e, li, n, s, *ps))) return rc;
+  } else {  // causal attention, query head i on key/value head i / (heads / kv_heads)
     AttnArgs a;
     a.q = s.q;
     a.k = s.k;
@@ -495,6 +584,8 @@ int exn_enc_open(const exn_enc_config* cfg, exn_enc** out) {
     ECK(static_cast<cudaError_t>(gemm_prepare()));
     ECK(static_cast<cudaError_t>(attention_prepare()));
     ECK(static_cast<cudaError_t>(gemm_thin_prepare()));
+    ECK(static_cast<cudaError_t>(packed_prepare()));
+    ECK(static_cast<cudaError_t>(cache_prepare()));
     ECK(cudaEventCreate(&e->ev[0]));
     ECK(cudaEventCreate(&e->ev[1]));
     // weights: one bf16 slab for every block's matrices, one fp32 array for the vectors
@@ -544,6 +635,8 @@ void exn_enc_close(exn_enc* e) {
   cudaSetDevice(e->cfg.device);
   if (e->st) cudaStreamSynchronize(e->st);
   if (e->scratch) cudaFree(e->scratch);
+  if (e->seqs) cudaFree(e->seqs);
+  if (e->attn_ws) cudaFree(e->attn_ws);
   if (e->slab) cudaFree(e->slab);
   if (e->vecs) cudaFree(e->vecs);
   if (e->embed) cudaFree(e->embed);
@@ -668,6 +761,53 @@ int exn_enc_load_gguf(exn_enc* e, const char* path) {
 
 namespace {
 
+// What a pass over N tokens of NSEQ sequences starts with: the checks of the ids, the scratch, the
+// inputs on the device, the embedded rows and the RoPE table.  POS: N x 3.
+int start_pass(exn_enc* e, const char* fn, const int32_t* ids, int n, const std::vector<int32_t>& pos, Scratch* s) {
+  for (int i = 0; i < n; ++i)
+    if (ids[i] < 0 || ids[i] >= e->cfg.vocab)
+      return efail(e, EXN_EINVAL, "%s: token %d is id %d, outside 0 .. %d", fn, i, ids[i], e->cfg.vocab - 1);
+  int rc;
+  if ((rc = ensure_scratch(e, n, s))) return rc;
+  ECK(cudaEventRecord(e->ev[0], e->st));
+  ECK(cudaMemcpyAsync(s->ids, ids, static_cast<size_t>(n) * 4, cudaMemcpyHostToDevice, e->st));
+  ECK(cudaMemcpyAsync(s->pos, pos.data(), pos.size() * 4, cudaMemcpyHostToDevice, e->st));
+  enc_embed_launch(e->embed, s->ids, s->x, n, e->cfg.width, e->st);
+  enc_rope_launch(s->pos, s->rope, n, e->cfg.theta, e->st);
+  ECK(cudaGetLastError());
+  return EXN_OK;
+}
+
+// the blocks of a pass
+int run_blocks(exn_enc* e, int n, const Scratch& s, const Pass* ps) {
+  bool normed = false;
+  int rc;
+  for (int li = 0; li < e->cfg.layers; ++li)
+    if ((rc = block(e, li, n, s, &normed, ps))) return rc;
+  return EXN_OK;
+}
+
+int finish_pass(exn_enc* e) {
+  ECK(cudaEventRecord(e->ev[1], e->st));
+  int rc;
+  if ((rc = enc_status(e))) return rc;
+  float ms = 0;
+  ECK(cudaEventElapsedTime(&ms, e->ev[0], e->ev[1]));
+  e->last_ms = ms;
+  return EXN_OK;
+}
+
+// the encoder's stream after the caller's queued work (NULL: CUDA's default stream)
+int after_stream(exn_enc* e, cudaStream_t user) {
+  cudaEvent_t ue;
+  ECK(cudaEventCreateWithFlags(&ue, cudaEventDisableTiming));
+  const cudaError_t r1 = cudaEventRecord(ue, user);
+  const cudaError_t r2 = r1 == cudaSuccess ? cudaStreamWaitEvent(e->st, ue, 0) : r1;
+  cudaEventDestroy(ue);
+  ECK(r2);
+  return EXN_OK;
+}
+
 // The pass of exn_enc_states: rows SKIP .. N-1 of the states into OUT, host memory or (DEVICE)
 // device memory of the encoder's device, the pass ordered after what USER's stream holds
 int run_states(exn_enc* e, const int32_t* ids, int n, const int32_t* positions, int skip, float* out, bool device,
@@ -675,9 +815,6 @@ int run_states(exn_enc* e, const int32_t* ids, int n, const int32_t* positions, 
   if (!e || !ids || !out) return efail(e, EXN_EINVAL, "exn_enc_states: null argument");
   if (n < 1 || n > kMaxTokens) return efail(e, EXN_EINVAL, "exn_enc_states: %d tokens (1 .. %d)", n, kMaxTokens);
   if (!exn_enc_weights_ready(e)) return efail(e, EXN_ENOWEIGHTS, "exn_enc_states: the encoder's weights are not loaded");
-  for (int i = 0; i < n; ++i)
-    if (ids[i] < 0 || ids[i] >= e->cfg.vocab)
-      return efail(e, EXN_EINVAL, "exn_enc_states: token %d is id %d, outside 0 .. %d", i, ids[i], e->cfg.vocab - 1);
   std::vector<int32_t> pos(static_cast<size_t>(n) * 3);
   for (int i = 0; i < n; ++i)
     for (int a = 0; a < 3; ++a) pos[3 * i + a] = positions ? positions[3 * i + a] : i;
@@ -685,32 +822,103 @@ int run_states(exn_enc* e, const int32_t* ids, int n, const int32_t* positions, 
   if (skip < 0 || skip >= n) return efail(e, EXN_EINVAL, "exn_enc_states: skip %d of %d tokens", skip, n);
   Scratch s;
   int rc;
-  if ((rc = ensure_scratch(e, n, &s))) return rc;
-  if (device) {  // after the caller's queued work (NULL: CUDA's default stream)
-    cudaEvent_t ue;
-    ECK(cudaEventCreateWithFlags(&ue, cudaEventDisableTiming));
-    const cudaError_t r1 = cudaEventRecord(ue, user);
-    const cudaError_t r2 = r1 == cudaSuccess ? cudaStreamWaitEvent(e->st, ue, 0) : r1;
-    cudaEventDestroy(ue);
-    ECK(r2);
-  }
-  ECK(cudaEventRecord(e->ev[0], e->st));
-  ECK(cudaMemcpyAsync(s.ids, ids, static_cast<size_t>(n) * 4, cudaMemcpyHostToDevice, e->st));
-  ECK(cudaMemcpyAsync(s.pos, pos.data(), pos.size() * 4, cudaMemcpyHostToDevice, e->st));
-  enc_embed_launch(e->embed, s.ids, s.x, n, e->cfg.width, e->st);
-  enc_rope_launch(s.pos, s.rope, n, e->cfg.theta, e->st);
-  ECK(cudaGetLastError());
-  bool normed = false;
-  for (int li = 0; li < e->cfg.layers; ++li)
-    if ((rc = block(e, li, n, s, &normed))) return rc;
+  if (device && (rc = after_stream(e, user))) return rc;
+  if ((rc = start_pass(e, "exn_enc_states", ids, n, pos, &s))) return rc;
+  if ((rc = run_blocks(e, n, s, nullptr))) return rc;
   const size_t w = e->cfg.width;
   ECK(cudaMemcpyAsync(out, s.x + static_cast<size_t>(skip) * w, static_cast<size_t>(n - skip) * w * 4,
                       device ? cudaMemcpyDeviceToDevice : cudaMemcpyDeviceToHost, e->st));
-  ECK(cudaEventRecord(e->ev[1], e->st));
-  if ((rc = enc_status(e))) return rc;
-  float ms = 0;
-  ECK(cudaEventElapsedTime(&ms, e->ev[0], e->ev[1]));
-  e->last_ms = ms;
+  return finish_pass(e);
+}
+
+// FN's body with the host running out of memory as an error of the call
+template <typename F>
+int guarded(exn_enc* e, const char* fn, F body) {
+  try {
+    return body();
+  } catch (const std::exception& x) {
+    return efail(e, EXN_ENOMEM, "%s: %s", fn, x.what());
+  }
+}
+
+// The passes of several sequences: exn_enc_states_packed (CACHE null) and exn_enc_extend.  COUNTS tokens
+// of each; OUT (host, or device memory with DEVICE) gets each sequence's rows after its first SKIP.
+int run_sequences(exn_enc* e, const char* fn, exn_enc_cache* cache, const int32_t* ids, int nseq, const int32_t* counts,
+                  const int32_t* positions, int skip, float* out, bool device, cudaStream_t user) {
+  if (!e || !ids || !counts || !out) return efail(e, EXN_EINVAL, "%s: null argument", fn);
+  if (nseq < 1 || skip < 0) return efail(e, EXN_EINVAL, "%s: %d sequences, skip %d", fn, nseq, skip);
+  if (!exn_enc_weights_ready(e)) return efail(e, EXN_ENOWEIGHTS, "%s: the encoder's weights are not loaded", fn);
+  std::vector<int32_t> seqs(2 * static_cast<size_t>(nseq) + 1);  // offsets [nseq + 1], lengths [nseq]
+  int64_t total = 0;
+  for (int i = 0; i < nseq; ++i) {
+    const int64_t before = cache ? cache->lens[i] : 0;
+    if (counts[i] < 0 || (counts[i] && skip >= counts[i]))
+      return efail(e, EXN_EINVAL, "%s: sequence %d has %d tokens (skip %d)", fn, i, counts[i], skip);
+    if (cache && before + counts[i] > static_cast<int64_t>(cache->ld) * kPage)
+      return efail(e, EXN_EINVAL, "%s: sequence %d has %lld tokens kept and %d new, room for %lld", fn, i,
+                   static_cast<long long>(before), counts[i], static_cast<long long>(cache->ld) * kPage);
+    seqs[i] = static_cast<int32_t>(total);
+    total += counts[i];
+    if (total > kMaxTokens) return efail(e, EXN_EINVAL, "%s: more than %d tokens", fn, kMaxTokens);
+    seqs[nseq + 1 + i] = static_cast<int32_t>(before + counts[i]);
+  }
+  seqs[nseq] = static_cast<int32_t>(total);
+  const int n = static_cast<int>(total);
+  if (n < 1) return efail(e, EXN_EINVAL, "%s: no token in any sequence", fn);
+  std::vector<int32_t> pos(static_cast<size_t>(n) * 3);
+  for (int i = 0; i < nseq; ++i)
+    for (int j = 0; j < counts[i]; ++j)
+      for (int a = 0; a < 3; ++a) {
+        const size_t t = 3 * (static_cast<size_t>(seqs[i]) + j) + a;
+        pos[t] = positions ? positions[t] : (cache ? cache->lens[i] : 0) + j;
+      }
+  ECK(cudaSetDevice(e->cfg.device));
+  int rc;
+  if (device && (rc = after_stream(e, user))) return rc;
+  if (seqs.size() > e->seqs_cap) {
+    if (e->seqs) cudaFree(e->seqs);
+    e->seqs = nullptr;
+    e->seqs_cap = 0;
+    ECK(cudaMalloc(&e->seqs, seqs.size() * 4));
+    e->seqs_cap = seqs.size();
+  }
+  Pass ps;
+  ps.nseq = nseq;
+  ps.offsets = e->seqs;
+  ps.lens = e->seqs + nseq + 1;
+  ps.cache = cache;
+  if (cache) {
+    const size_t need = cache_attention_workspace(cache_args(cache, 0, nullptr), e->cfg.heads, n);
+    if (need > e->attn_ws_cap) {
+      if (e->attn_ws) cudaFree(e->attn_ws);
+      e->attn_ws = nullptr;
+      e->attn_ws_cap = 0;
+      ECK(cudaMalloc(&e->attn_ws, need));
+      e->attn_ws_cap = need;
+    }
+    ps.ws = e->attn_ws;
+    ps.ws_bytes = e->attn_ws_cap;
+  }
+  Scratch s;
+  if ((rc = start_pass(e, fn, ids, n, pos, &s))) return rc;
+  ECK(cudaMemcpyAsync(e->seqs, seqs.data(), seqs.size() * 4, cudaMemcpyHostToDevice, e->st));
+  if ((rc = run_blocks(e, n, s, &ps))) return rc;
+  const size_t w = e->cfg.width;
+  const cudaMemcpyKind kind = device ? cudaMemcpyDeviceToDevice : cudaMemcpyDeviceToHost;
+  if (skip == 0) {
+    ECK(cudaMemcpyAsync(out, s.x, n * w * 4, kind, e->st));
+  } else {
+    float* dst = out;
+    for (int i = 0; i < nseq; ++i) {
+      if (!counts[i]) continue;
+      const size_t rows = counts[i] - skip;
+      ECK(cudaMemcpyAsync(dst, s.x + (static_cast<size_t>(seqs[i]) + skip) * w, rows * w * 4, kind, e->st));
+      dst += rows * w;
+    }
+  }
+  if ((rc = finish_pass(e))) return rc;
+  if (cache)
+    for (int i = 0; i < nseq; ++i) cache->lens[i] += counts[i];
   return EXN_OK;
 }
 
@@ -727,6 +935,82 @@ int exn_enc_states_device(exn_enc* e, const int32_t* ids, int n, const int32_t* 
   return run_states(e, ids, n, positions, skip, d_states, true, static_cast<cudaStream_t>(stream));
 }
 
+int exn_enc_states_packed(exn_enc* e, const int32_t* ids, int nseq, const int32_t* counts, const int32_t* positions,
+                          float* states) {
+  static const char fn[] = "exn_enc_states_packed";
+  return guarded(e, fn, [&] { return run_sequences(e, fn, nullptr, ids, nseq, counts, positions, 0, states, false, nullptr); });
+}
+
+int exn_enc_states_packed_device(exn_enc* e, const int32_t* ids, int nseq, const int32_t* counts,
+                                 const int32_t* positions, int skip, float* d_states, void* stream) {
+  static const char fn[] = "exn_enc_states_packed_device";
+  return guarded(e, fn, [&] {
+    return run_sequences(e, fn, nullptr, ids, nseq, counts, positions, skip, d_states, true,
+                         static_cast<cudaStream_t>(stream));
+  });
+}
+
+int exn_enc_cache_open(exn_enc* e, int nseq, int max_tokens, exn_enc_cache** out) {
+  if (!e || !out) return efail(e, EXN_EINVAL, "exn_enc_cache_open: null argument");
+  *out = nullptr;
+  const int64_t ld = (static_cast<int64_t>(max_tokens) + kPage - 1) / kPage;
+  if (nseq < 1 || max_tokens < 1 || ld * nseq * e->cfg.kv_heads > 0x7fffffff)
+    return efail(e, EXN_EINVAL, "exn_enc_cache_open: %d sequences of %d tokens", nseq, max_tokens);
+  ECK(cudaSetDevice(e->cfg.device));
+  exn_enc_cache* c = new (std::nothrow) exn_enc_cache();
+  if (!c) return efail(e, EXN_ENOMEM, "exn_enc_cache_open: out of memory");
+  c->owner = e;
+  c->device = e->cfg.device;
+  c->nseq = nseq;
+  c->ld = static_cast<int>(ld);
+  c->layers = e->cfg.layers;
+  c->kv_heads = e->cfg.kv_heads;
+  const int rc = guarded(e, "exn_enc_cache_open", [&]() -> int {
+    c->lens.assign(nseq, 0);
+    const size_t heads = static_cast<size_t>(ld) * nseq * c->kv_heads * 2 * c->layers;
+    std::vector<int32_t> table(static_cast<size_t>(ld) * nseq);
+    for (size_t i = 0; i < table.size(); ++i) table[i] = static_cast<int32_t>(i);
+    ECK(cudaMalloc(&c->codes, heads * kPage * kHeadDim));
+    ECK(cudaMalloc(&c->scales, heads * 4));
+    ECK(cudaMalloc(&c->table, table.size() * 4));
+    ECK(cudaMemcpy(c->table, table.data(), table.size() * 4, cudaMemcpyHostToDevice));
+    return EXN_OK;
+  });
+  if (rc) {
+    exn_enc_cache_close(c);
+    return rc;
+  }
+  *out = c;
+  return EXN_OK;
+}
+
+void exn_enc_cache_close(exn_enc_cache* c) {
+  if (!c) return;
+  cudaSetDevice(c->device);
+  if (c->codes) cudaFree(c->codes);
+  if (c->scales) cudaFree(c->scales);
+  if (c->table) cudaFree(c->table);
+  delete c;
+}
+
+int exn_enc_cache_length(const exn_enc_cache* c, int seq) { return c && seq >= 0 && seq < c->nseq ? c->lens[seq] : -1; }
+
+int exn_enc_cache_trim(exn_enc* e, exn_enc_cache* c, int seq, int tokens) {
+  if (!e || !c || c->owner != e) return efail(e, EXN_EINVAL, "exn_enc_cache_trim: null argument, or another encoder's cache");
+  if (seq < 0 || seq >= c->nseq || tokens < 0 || tokens > c->lens[seq])
+    return efail(e, EXN_EINVAL, "exn_enc_cache_trim: sequence %d of %d to %d tokens of %d", seq, c->nseq, tokens,
+                 seq >= 0 && seq < c->nseq ? c->lens[seq] : 0);
+  c->lens[seq] = tokens;
+  return EXN_OK;
+}
+
+int exn_enc_extend(exn_enc* e, exn_enc_cache* c, const int32_t* ids, const int32_t* counts, const int32_t* positions,
+                   float* states) {
+  if (!e || !c || c->owner != e) return efail(e, EXN_EINVAL, "exn_enc_extend: null argument, or another encoder's cache");
+  static const char fn[] = "exn_enc_extend";
+  return guarded(e, fn, [&] { return run_sequences(e, fn, c, ids, c->nseq, counts, positions, 0, states, false, nullptr); });
+}
+
 int exn_enc_release(exn_enc* e) {
   if (!e) return efail(e, EXN_EINVAL, "exn_enc_release: null handle");
   ECK(cudaSetDevice(e->cfg.device));
@@ -734,6 +1018,12 @@ int exn_enc_release(exn_enc* e) {
   if (e->scratch) ECK(cudaFree(e->scratch));
   e->scratch = nullptr;
   e->cap = 0;
+  if (e->seqs) ECK(cudaFree(e->seqs));
+  e->seqs = nullptr;
+  e->seqs_cap = 0;
+  if (e->attn_ws) ECK(cudaFree(e->attn_ws));
+  e->attn_ws = nullptr;
+  e->attn_ws_cap = 0;
   return EXN_OK;
 }
 

@@ -171,9 +171,6 @@ int cache_write_launch(const CacheArgs& c, int f16, const int* offsets, long lon
                        const void* v, long long ld_v, int* d_status, cudaStream_t st);
 int cache_read_launch(const CacheArgs& c, int f16, const int* offsets, long long rows, void* k, long long ld_k,
                       void* v, long long ld_v, int* d_status, cudaStream_t st);
-// every position of every sequence: position j of sequence s to row s * table_ld * 64 + j of K and V
-// [nseq * table_ld * 64][kv_heads * 128]
-int cache_dense_launch(const CacheArgs& c, int f16, void* k, void* v, int* d_status, cudaStream_t st);
 struct CacheAttnArgs {
   CacheArgs c;
   int f16 = 0, heads = 0;
@@ -185,8 +182,9 @@ struct CacheAttnArgs {
   long long ld_out = 0;
   float scale_log2 = 0.f;
 };
-// few rows a sequence: one pass over the codes on CUDA's warp-level MMA, the keys split over clusters
-int cache_attend_launch(const CacheAttnArgs& a, int sms, int* d_status, cudaStream_t st);
+// WS: cache_attention_workspace's bytes, 16-byte aligned.  0, -1 (size), -4 (tensor map) or a cudaError_t.
+int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, int* d_status, cudaStream_t st);
+size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows);
 int cache_prepare();
 
 // C = A . (q d)^T with the weights as Q8_0 (gemm_q8.cu): QS int8 [N][K], DK the fp16 scales laid out

@@ -83,6 +83,7 @@ def lib():
     fp = ctypes.POINTER(ctypes.c_float)
     vp = ctypes.c_void_p
     i64 = ctypes.c_int64
+    i32p = ctypes.POINTER(ctypes.c_int32)
     sigs = {
         "exn_abi_version": (ctypes.c_int, []),
         "exn_default_config": (None, [ctypes.POINTER(Config)]),
@@ -125,6 +126,13 @@ def lib():
                                           ctypes.POINTER(ctypes.c_int32), fp]),
         "exn_enc_states_device": (ctypes.c_int, [H, ctypes.POINTER(ctypes.c_int32), ctypes.c_int,
                                                  ctypes.POINTER(ctypes.c_int32), ctypes.c_int, vp, vp]),
+        "exn_enc_states_packed": (ctypes.c_int, [H, i32p, ctypes.c_int, i32p, i32p, fp]),
+        "exn_enc_states_packed_device": (ctypes.c_int, [H, i32p, ctypes.c_int, i32p, i32p, ctypes.c_int, vp, vp]),
+        "exn_enc_cache_open": (ctypes.c_int, [H, ctypes.c_int, ctypes.c_int, ctypes.POINTER(H)]),
+        "exn_enc_cache_close": (None, [H]),
+        "exn_enc_cache_trim": (ctypes.c_int, [H, H, ctypes.c_int, ctypes.c_int]),
+        "exn_enc_cache_length": (ctypes.c_int, [H, ctypes.c_int]),
+        "exn_enc_extend": (ctypes.c_int, [H, H, i32p, i32p, i32p, fp]),
         "exn_enc_release": (ctypes.c_int, [H]),
         "exn_test_enc_last_ms": (ctypes.c_int, [H, ctypes.POINTER(ctypes.c_double)]),
         "exn_test_enc_weights_digest": (ctypes.c_int, [H, ctypes.POINTER(ctypes.c_uint64)]),
@@ -497,6 +505,43 @@ class Encoder:
                                              pos.ctypes.data_as(ip) if pos is not None else None, skip,
                                              ctypes.c_void_p(d_states), ctypes.c_void_p(stream)))
 
+    @staticmethod
+    def _pack(prompts, positions):
+        """Lists of token ids (and of (n, 3) positions) packed: ids, counts, positions or None."""
+        seqs = [np.ascontiguousarray(p, dtype=np.int32).ravel() for p in prompts]
+        counts = np.array([len(p) for p in seqs], dtype=np.int32)
+        ids = np.concatenate(seqs) if seqs else np.zeros(0, dtype=np.int32)
+        if positions is None:
+            return ids, counts, None
+        pos = [np.ascontiguousarray(p, dtype=np.int32) for p in positions]
+        if len(pos) != len(seqs) or any(p.shape != (n, 3) for p, n in zip(pos, counts)):
+            raise ExnError(1, "positions must be one (n, 3) array a prompt")
+        return ids, counts, np.ascontiguousarray(np.concatenate(pos))
+
+    def states_packed(self, prompts, positions=None):
+        """encoder-states of several prompts in one pass: a list of (n, width) float32 arrays.  PROMPTS: token
+        ids of each; POSITIONS: an (n, 3) array for each, or None."""
+        ids, counts, pos = self._pack(prompts, positions)
+        out = np.empty((len(ids), self.cfg.width), dtype=np.float32)
+        ip = ctypes.POINTER(ctypes.c_int32)
+        self._ck(lib().exn_enc_states_packed(self.h, ids.ctypes.data_as(ip), len(counts), counts.ctypes.data_as(ip),
+                                             pos.ctypes.data_as(ip) if pos is not None else None, _fp(out)))
+        return np.split(out, np.cumsum(counts)[:-1])
+
+    def states_packed_device(self, prompts, d_states, positions=None, skip=0, stream=None):
+        """The same into device memory (a pointer): each prompt's rows SKIP.., one after another; prompts of
+        one length give the contexts of Dit.generate_device."""
+        ids, counts, pos = self._pack(prompts, positions)
+        ip = ctypes.POINTER(ctypes.c_int32)
+        self._ck(lib().exn_enc_states_packed_device(self.h, ids.ctypes.data_as(ip), len(counts),
+                                                    counts.ctypes.data_as(ip),
+                                                    pos.ctypes.data_as(ip) if pos is not None else None, skip,
+                                                    ctypes.c_void_p(d_states), ctypes.c_void_p(stream)))
+
+    def cache(self, nseq, max_tokens):
+        """Room for the keys and values of NSEQ growing prompts (an EncoderCache)."""
+        return EncoderCache(self, nseq, max_tokens)
+
     def release(self):
         self._ck(lib().exn_enc_release(self.h))
 
@@ -509,6 +554,54 @@ class Encoder:
         d = ctypes.c_uint64()
         self._ck(lib().exn_test_enc_weights_digest(self.h, ctypes.byref(d)))
         return d.value
+
+
+class EncoderCache:
+    """Kept keys and values (8 bits) of NSEQ prompts of up to MAX_TOKENS tokens each on ENCODER."""
+
+    def __init__(self, encoder, nseq, max_tokens):
+        h = ctypes.c_void_p()
+        encoder._ck(lib().exn_enc_cache_open(encoder.h, nseq, max_tokens, ctypes.byref(h)))
+        self.h = h
+        self.encoder = encoder
+        self.nseq = nseq
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().exn_enc_cache_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+    def extend(self, tokens, positions=None):
+        """More tokens of every prompt (NSEQ lists of ids, empty ones among them): their states, a list of
+        (n, width) float32 arrays."""
+        e = self.encoder
+        if len(tokens) != self.nseq:
+            raise ExnError(1, "tokens of %d prompts, the cache has %d" % (len(tokens), self.nseq))
+        ids, counts, pos = e._pack(tokens, positions)
+        out = np.empty((len(ids), e.cfg.width), dtype=np.float32)
+        ip = ctypes.POINTER(ctypes.c_int32)
+        e._ck(lib().exn_enc_extend(e.h, self.h, ids.ctypes.data_as(ip), counts.ctypes.data_as(ip),
+                                   pos.ctypes.data_as(ip) if pos is not None else None, _fp(out)))
+        return np.split(out, np.cumsum(counts)[:-1])
+
+    def trim(self, seq, tokens):
+        """Keep the first TOKENS tokens of prompt SEQ."""
+        self.encoder._ck(lib().exn_enc_cache_trim(self.encoder.h, self.h, seq, tokens))
+
+    def lengths(self):
+        return [lib().exn_enc_cache_length(self.h, s) for s in range(self.nseq)]
 
 
 class Attention:

@@ -241,7 +241,40 @@ int exn_enc_states(exn_enc* e, const int32_t* ids, int n, const int32_t* positio
 int exn_enc_states_device(exn_enc* e, const int32_t* ids, int n, const int32_t* positions, int skip,
                           float* d_states, void* stream);
 
-/* The encoder's scratch freed (the weights stay). */
+/* Several prompts in one pass, for the pictures of exn_generate_batch / exn_generate_device: IDS holds
+ * COUNTS[0] token ids of the first prompt, then COUNTS[1] of the second, .. (32768 in all; a count may
+ * be 0), POSITIONS (or NULL: (i, i, i) within each prompt) and STATES likewise.  Every prompt's states are those
+ * of a pass of its own; the weights are read once for all of them. */
+int exn_enc_states_packed(exn_enc* e, const int32_t* ids, int nseq, const int32_t* counts, const int32_t* positions,
+                          float* states);
+
+/* The same into device memory of the encoder's device, each prompt's rows SKIP .. after the last one's
+ * (every prompt that has tokens has more than SKIP): with equal counts, the contexts of
+ * exn_generate_device.  Ordered and complete as exn_enc_states_device. */
+int exn_enc_states_packed_device(exn_enc* e, const int32_t* ids, int nseq, const int32_t* counts,
+                                 const int32_t* positions, int skip, float* d_states, void* stream);
+
+/* Prompts that grow: the keys and values of NSEQ sequences of up to MAX_TOKENS tokens (rounded up to a
+ * multiple of 64) are kept in 8 bits (the cache of exn_attn_cache_write below, every block's), so that a
+ * token is encoded once: the system turn that every prompt starts with, a prompt that is edited from some
+ * word on.  The cache belongs to the encoder it was opened on, is used by one thread at a time with it,
+ * and may be closed before or after it.  Its memory: 2 * layers * kv_heads * 128 bytes a token (73.7 KB
+ * for Qwen3-VL-8B). */
+typedef struct exn_enc_cache exn_enc_cache;
+int exn_enc_cache_open(exn_enc* e, int nseq, int max_tokens, exn_enc_cache** out);
+void exn_enc_cache_close(exn_enc_cache* c);
+
+/* COUNTS[s] more tokens of every sequence (0: none), packed in IDS, POSITIONS (NULL: a token's place in its
+ * sequence, thrice) and STATES as exn_enc_states_packed's.  A token's state is exn_enc_states's but for
+ * the rounding of the keys and values it attends to, its own among them. */
+int exn_enc_extend(exn_enc* e, exn_enc_cache* c, const int32_t* ids, const int32_t* counts, const int32_t* positions,
+                   float* states);
+
+/* Keep the first TOKENS tokens of sequence SEQ (0: start it anew); its tokens now, or -1. */
+int exn_enc_cache_trim(exn_enc* e, exn_enc_cache* c, int seq, int tokens);
+int exn_enc_cache_length(const exn_enc_cache* c, int seq);
+
+/* The encoder's scratch freed (the weights and open caches stay). */
 int exn_enc_release(exn_enc* e);
 
 /* ---- Attention on device memory: the language model's operators that the prompt encoder is made of,
