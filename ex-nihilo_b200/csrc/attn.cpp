@@ -286,7 +286,7 @@ int exn_attn_cache_workspace(exn_attn* a, const exn_kv_cache* cache, int heads, 
   CacheArgs c;
   if ((rc = check_cache(a, fn, cache, &c)) || (rc = check_heads(a, fn, heads, c.kv_heads))) return rc;
   if (!bytes || rows < 0 || rows > kMaxRows) return afail(a, EXN_EINVAL, "%s: null result, or %lld rows", fn, static_cast<long long>(rows));
-  *bytes = c.nseq ? cache_attention_workspace(c, heads, rows) : 0;
+  *bytes = c.nseq ? cache_attention_workspace(c, heads, rows, a->sms) : 0;
   return EXN_OK;
 }
 
@@ -305,7 +305,7 @@ int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int 
   if ((rc = check_matrix(a, fn, "q", q, &ld_q, heads)) || (rc = check_matrix(a, fn, "out", out, &ld_out, heads)))
     return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const size_t need = cache_attention_workspace(p.c, heads, rows);
+  const size_t need = cache_attention_workspace(p.c, heads, rows, a->sms);
   if (need > workspace_bytes || (need && !workspace))
     return afail(a, EXN_EINVAL, "%s: a workspace of %zu bytes, %zu needed", fn, workspace ? workspace_bytes : 0, need);
   if (need && !aligned(workspace, 256)) return afail(a, EXN_EINVAL, "%s: the workspace is not 256-byte aligned", fn);

@@ -13,6 +13,9 @@
 // bits): what the cache stands for does not depend on who reads it.  A page
 // that is given an infinity or a NaN gets the scale NaN and makes NaN of what
 // is read from it until it starts anew at its first position.
+#include <atomic>
+#include <random>
+
 #include "exn_device.cuh"
 #include "exn_internal.h"
 
@@ -256,32 +259,48 @@ __global__ void __launch_bounds__(256) k_cache_read(const CacheArgs c, const int
 
 // ---- attention of a few rows over the codes
 //
-// One cluster = one tile of up to 8 NT query rows (tokens times the query heads that read one
-// key/value head) of a sequence; its WARPS * CTAs warps take the sequence's pages in turn, each with
-// its own running maximum, sum and output, joined at the end through shared memory and the cluster's.
-// Bound by the codes' bytes (a code takes part in 4 g c operations), as long as the conversions to
-// 16 bits keep up: they are the bulk of the instructions, so
-//   * both products run on fp16 MMAs (m16n8k16), whichever type q has: an int8 code becomes fp16
-//     exactly with one byte permute and one subtraction a pair (1024 + (code + 128) is fp16 0x6400 |
-//     byte); a row of q is scaled by a power of two to lie below 2^15 (bf16's 8 bits fit fp16's 11;
-//     what is 2^-29 of the row's largest is lost), P is at most 1;
+// An item is a tile of up to 8 NT query rows (tokens times the query heads that read one key/value head)
+// of one sequence; its work is the sequence's half pages ("spans", 32 positions) and SETUP more for what an
+// item costs by itself.  The work of all items, laid end to end, is cut into equal parts, one a CTA, so a
+// launch is one wave whatever the lengths: a long sequence is shared by many CTAs, short ones share a CTA.
+// In a CTA one warp brings the data and the others compute: the producer finds the CTA's part of the work,
+// turns each item's rows of q into the MMA's operand and streams the spans with TMA, dealt out to the
+// other warps in turn, through a ring of 4 KB tiles each (K_0 V_0 K_1 ..; 128-byte swizzle, so that the
+// reads below touch every bank once); it runs ahead from one item into the next.  Each computing warp has
+// its own running maximum, sum and output, joined through shared memory at the item's end.  An item that is
+// cut leaves each CTA's joined part in the workspace and counts it; the CTA whose part is the last (nobody
+// waits) adds the parts in their order, so the bits do not depend on who it was.  The count is kept under
+// the launch's tag, a number that no other launch of the process has, so whatever the workspace held before
+// is not taken for one.
+//
+// Bound by the codes' bytes (a code takes part in 4 g c operations) as long as the instructions keep up.
+// A byte permute, a logical operation and a paired fp16 one each take a scheduler two clocks a warp, an
+// MMA eight, so what turns codes into operands is what counts:
 //   * codes are the 16-row operand and the queries the 8 columns: S^T = K Q^T, O^T = V^T P^T, so 8
-//     rows of queries waste nothing; P^T turns from the first product's layout to the second's with
-//     movmatrix;
-//   * the scales stay out of the products: 2^ek multiplies the scores, 2^ev the page's fp32 sums.
-// Each warp streams its pages with TMA through a ring of its own (K_0 V_0 K_1 ..., 8 KB each, 128-byte
-// swizzle: the 16-byte reads below touch every bank once) and re-fills a slot as soon as it has
-// read it.
-constexpr int MAX_CLUSTER = 16;
+//     rows of queries waste nothing;
+//   * K's codes are multiplied as they are (m16n8k32, s8): a row of q is two int8 numbers, q = 2^a (hi +
+//     lo / 256) with 2^a the smallest power of two that |q| <= 127 2^a allows.  The sums are exact; q
+//     itself is, for elements of 1/128 (bf16) or 1/16 (fp16) of the row's largest and more, and off by
+//     at most 2^-15 of the largest below;
+//   * V's codes become fp16 (m16n8k16), exactly: ldmatrix.trans brings a position pair's codes of two
+//     dims into one register, from which 1024 + (code + 128) is 0x6400 | byte; the subtraction of 1152 is a
+//     fused multiply-add that scales by 2^ev as well, relative to the unit the warp's sums are in, so
+//     the product adds to the sums in place.  P is fp16, at most 2^8: the sums are rescaled only
+//     when the row maximum grows by more than 2^8;
+//   * P^T turns from the first product's layout to the second's with movmatrix.
+constexpr int SPAN = 32;                  // positions a warp takes at a time
+constexpr int SPAN_BYTES = SPAN * 128;
+constexpr int SETUP = 12;                 // what an item costs besides its spans, in spans
+constexpr int MIN_PART = 16 + SETUP;      // the least work worth a CTA that may take several items
 
-template <int WARPS, int NT>
+// Tiles of 8 rows (NT 1): two CTAs of 5 + 1 warps an SM, 168 registers a thread; of 16 rows, whose sums take
+// twice the registers, one of 7 + 1
+template <int NT>
 struct AttendCfg {
-  static constexpr int SLOTS = 3;
-  static constexpr int RING = WARPS * SLOTS * PAGE_BYTES;
-  static constexpr int ROWS = 8 * NT;
-  static constexpr int OFF_BAR = RING;
-  static constexpr int OFF_JOIN = OFF_BAR + WARPS * SLOTS * 8 + 64;  // the CTA's joined m, l [ROWS] each
-  static constexpr int SMEM = OFF_JOIN + 2 * ROWS * 4 + 1024;
+  static constexpr int WARPS = NT == 1 ? 5 : 7, CTAS = NT == 1 ? 2 : 1, ROWS = 8 * NT, THREADS = (WARPS + 1) * 32;
+  static constexpr int SLOTS = 4;
+  static constexpr int RING = WARPS * SLOTS * SPAN_BYTES, JOIN = WARPS * ROWS * 512;
+  static constexpr int SMEM = RING + JOIN + 1024;
 };
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -294,453 +313,807 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-// two pairs of biased codes (code + 128) to fp16: bytes 0, 1 and bytes 2, 3
-__device__ __forceinline__ uint32_t codes_lo(uint32_t u) {
-  const uint32_t h = __byte_perm(u, 0x64646464u, 0x4140);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&r);
+// d = a b + the integer whose bits are the float 1.5 * 2^23: the float of d's bits less that is the product
+__device__ __forceinline__ void mma16832_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0x4b400000));
 }
-__device__ __forceinline__ uint32_t codes_hi(uint32_t u) {
-  const uint32_t h = __byte_perm(u, 0x64646464u, 0x4342);
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+// two of four biased codes (code + 128), bytes 0 and 2 or 1 and 3, as fp16 code * r: (1024 + byte) r - 1152 r, exact
+__device__ __forceinline__ uint32_t v_pair(uint32_t u, uint32_t sel, __half2 r, __half2 c) {
+  const uint32_t h = __byte_perm(u, 0x64646464u, sel);
+  const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&h), r, c);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+constexpr uint32_t EVEN = 0x4240, ODD = 0x4341;
+// four 8 x 8 matrices of 16-bit elements, transposed; a lane's address is a row of one of them
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                : "r"(addr)
                : "memory");
   return v;
 }
-__device__ __forceinline__ float ld_cluster_f(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void fence_acq_rel() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
+
+// The counts of an item's parts, tag + parts so far.  Before a launch there is 0, what the last part leaves, or
+// anything that is not the launch's tag.  The CTA that the item begins in raises it to the tag when it
+// starts; a part that finds no tag all the same (it came earlier, or there was something larger) puts it
+// there.
+__device__ __forceinline__ bool tagged(unsigned long long v, unsigned long long tag) { return (v & ~0xffffull) == tag; }
+__device__ __forceinline__ void start_count(unsigned long long* at, unsigned long long tag) {
+  asm volatile("red.relaxed.gpu.global.max.u64 [%0], %1;" ::"l"(at), "l"(tag) : "memory");
 }
-__device__ __forceinline__ uint32_t cluster_nctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
+// one more part: how many there were before
+__device__ __forceinline__ int count_part(unsigned long long* at, unsigned long long tag) {
+  unsigned long long v = atomicAdd(at, 1ull);
+  while (!tagged(v, tag)) {  // a few times at most: only the item's parts change it
+    const unsigned long long got = atomicCAS(at, v + 1, tag + 1);
+    if (got == v + 1) return 0;
+    v = tagged(got, tag) ? atomicAdd(at, 1ull) : got - 1;
+  }
+  return static_cast<int>(v & 0xffffull);
 }
 
-template <bool F16, int WARPS, int NT>
-__global__ void __launch_bounds__(WARPS * 32)
+// whether the phase of parity PARITY is complete; never waits
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// How a launch's work is cut, and its workspace
+struct AttendPlan {
+  int nt;                     // tiles of 8 nt rows
+  int hpt, head_tiles, tpt;   // heads and tokens a tile, tiles of a key/value head's query heads
+  int ctas;
+  unsigned long long tag;     // its low 16 bits are 0
+  // [ctas]: the parts of the item that begins in the CTA's work and goes on behind it, counted
+  unsigned long long* count;
+  // part 2 c: of the item that began before CTA c's work, 2 c + 1: of the one that goes on behind it
+  float* part;                // [2 ctas][ROWS][132]: o unnormalised, m, l
+};
+
+// A CTA's part of an item
+struct Seg {
+  int row0, tok, head0, nh;   // first row, tokens, first head, heads
+  int kvh, pos0;              // key/value head, position of the first row
+  int sp0, n, spans, item;    // spans sp0 .. sp0 + n - 1 of the item's; where it begins in the work
+};
+
+template <int NT>
+struct AttendShared {
+  using C = AttendCfg<NT>;
+  uint64_t full[C::WARPS][C::SLOTS], empty[C::WARPS][C::SLOTS];  // the rings
+  uint64_t seg_full[2], seg_empty[2];
+  Seg seg[2];                                    // n 0: no more
+  uint32_t q[2][2][C::ROWS][32];                 // [segment][hi, lo][row]: 128 codes
+  float q_scale[2][C::ROWS];                     // 2^a scale log2(e)
+  float4 meta[C::WARPS][2];                      // of a warp's span: K's and V's scale, first position (bits)
+  float m[C::WARPS][C::ROWS], l[C::WARPS][C::ROWS];
+  int part_len, lead, taken, abort_word;
+};
+
+// ---- the producer warp
+template <bool F16, int NT>
+__device__ __forceinline__ void attend_produce(const CUtensorMap* tmK, const CUtensorMap* tmV, const CacheAttnArgs& p,
+                                               const AttendPlan& plan, AttendShared<NT>& sh, uint8_t* ring, int* status) {
+  using C = AttendCfg<NT>;
+  constexpr int ROWS = C::ROWS, WARPS = C::WARPS, SLOTS = C::SLOTS;
+  const int lane = threadIdx.x & 31;
+  const int kv = p.c.kv_heads, g = p.heads / kv, per = plan.head_tiles * kv;
+  volatile int* abort_flag = &sh.abort_word;
+
+  // ---- this CTA's part of the work, [f, fend)
+  auto spans_of = [](int len) { return max(1, (len + SPAN - 1) / SPAN); };
+  // the items of a sequence of rows a .. b - 1; 0 for one whose numbers are out of range
+  auto items_of = [&](int a, int b, int len) -> int {
+    if (a < 0 || b < a || b > p.rows || len < 0 || len > static_cast<long long>(p.c.table_ld) * kPage) {
+      if (blockIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
+      return 0;
+    }
+    return (plan.tpt == 1 ? b - a : (b - a + plan.tpt - 1) / plan.tpt) * per;
+  };
+  const int chunk = (p.c.nseq + 31) / 32;  // a run of sequences a lane
+  const int s_lo = min(p.c.nseq, lane * chunk), s_hi = min(p.c.nseq, s_lo + chunk);
+  long long lane_work = 0;
+  int items = 0, longest = 0, start = 0, end = 0, len = 0;  // start, end, len: the lane's first sequence's
+  for (int s = s_lo; s < s_hi; ++s) {
+    const int a = p.offsets[s], b = p.offsets[s + 1], l = p.c.lens[s];
+    const int n = items_of(a, b, l);
+    items += n;
+    lane_work += static_cast<long long>(n) * (spans_of(l) + SETUP);
+    if (n) longest = max(longest, spans_of(l));
+    if (s == s_lo) {
+      start = a;
+      end = b;
+      len = l;
+    }
+  }
+  bool work_here = true;
+  if (__any_sync(0xffffffffu, lane_work >= (1ll << 26))) {  // 2^26 spans are 512 GB of codes
+    if (lane == 0) atomicOr(status, STATUS_BAD_ARG);
+    work_here = false;
+  }
+  const int work = static_cast<int>(lane_work);
+  int work_to = work, items_to = items;  // up to and with this lane's
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, work_to, o), y = __shfl_up_sync(0xffffffffu, items_to, o);
+    if (lane >= o) {
+      work_to += x;
+      items_to += y;
+    }
+    longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+  }
+  const int all_work = __shfl_sync(0xffffffffu, work_to, 31), all_items = __shfl_sync(0xffffffffu, items_to, 31);
+  // Equal parts of the work end to end, of at least MIN_PART; or, when the items are so few that each can have
+  // CTAs of its own and the longest one's parts are no longer for it, whole CTAs an item (a span a warp at
+  // least): no CTA then takes more than one item.
+  int part_len = max(MIN_PART, (all_work + plan.ctas - 1) / plan.ctas);
+  int stride = 0;  // an item's length when it has CTAs of its own: so many times part_len
+  if (all_items > 0 && all_items <= plan.ctas) {
+    const int each = min(plan.ctas / all_items, (longest + WARPS - 1) / WARPS);
+    const int own = (longest + each - 1) / each;
+    if (own <= part_len) {
+      part_len = own;
+      stride = own * each;
+    }
+  }
+  const int lead = stride ? 0 : SETUP;
+  auto item_len = [&](int spans) { return stride ? stride : spans + SETUP; };
+  const long long f64 = static_cast<long long>(part_len) * blockIdx.x;
+  const int total = stride ? all_items * stride : all_work;  // below 2^31: stride < longest + ctas, items <= ctas
+  work_here = work_here && f64 < total;
+  int f = work_here ? static_cast<int>(f64) : 0;
+  const int fend = work_here ? min(f + part_len, total) : 0;
+  int seq = s_lo, count = end - start;
+  int base = stride ? (items_to - items) * stride : work_to - work;
+  if (work_here) {
+    const bool here = f >= base && f < base + (stride ? items * stride : work);
+    if (here)
+      while (true) {
+        const int w = items_of(start, start + count, len) * item_len(spans_of(len));
+        if (f < base + w) break;
+        base += w;
+        ++seq;
+        start = p.offsets[seq];
+        count = p.offsets[seq + 1] - start;
+        len = p.c.lens[seq];
+      }
+    const int owner = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    seq = __shfl_sync(0xffffffffu, seq, owner);
+    start = __shfl_sync(0xffffffffu, start, owner);
+    count = __shfl_sync(0xffffffffu, count, owner);
+    len = __shfl_sync(0xffffffffu, len, owner);
+    base = __shfl_sync(0xffffffffu, base, owner);
+    if (lane == 0) start_count(plan.count + blockIdx.x, plan.tag);
+  }
+  // the next part of an item: its description (n 0: no more), the row of the table, the positions seen
+  const int* table = nullptr;
+  int seen = 0;
+  auto advance = [&]() -> Seg {
+    Seg x = {};
+    while (f < fend) {
+      const int spans = spans_of(len), whole_len = item_len(spans);
+      const int w = items_of(start, start + count, len) * whole_len;
+      if (f >= base + w) {  // the next sequence
+        base += w;
+        ++seq;
+        start = p.offsets[seq];
+        count = p.offsets[seq + 1] - start;
+        len = p.c.lens[seq];
+        continue;
+      }
+      const unsigned idx = static_cast<unsigned>(f - base) / static_cast<unsigned>(whole_len);
+      x.item = base + static_cast<int>(idx) * whole_len;  // its spans begin LEAD later
+      const int f_next = min(x.item + whole_len, fend);
+      x.sp0 = max(f - x.item - lead, 0);
+      x.n = min(max(f_next - x.item - lead, 0), spans) - x.sp0;
+      f = f_next;
+      if (x.n <= 0) {  // none of its spans lie here
+        x.n = 0;
+        continue;
+      }
+      const unsigned tile = idx < static_cast<unsigned>(per) ? 0u : idx / static_cast<unsigned>(per), rest = idx - tile * per;
+      const int ht = plan.head_tiles == 1 ? 0 : rest / static_cast<unsigned>(kv);
+      const int t0 = static_cast<int>(tile) * plan.tpt;  // first token of the tile; token t is position t + len - count
+      x.spans = spans;
+      x.kvh = rest - ht * kv;
+      x.row0 = start + t0;
+      x.tok = min(plan.tpt, count - t0);
+      x.head0 = x.kvh * g + ht * plan.hpt;
+      x.nh = min(plan.hpt, g - ht * plan.hpt);
+      x.pos0 = t0 + len - count;
+      seen = x.pos0 + x.tok;
+      table = p.c.table + static_cast<long long>(seq) * p.c.table_ld;
+      break;
+    }
+    return x;
+  };
+  // page and scales of span I of a segment; a span that nothing of the tile sees or whose page is not the pool's
+  // has the scale -1 and is left out
+  struct Ids {
+    int pid;
+    float sk, sv;
+  };
+  auto fetch_ids = [&](const Seg& x, const int* tab, int upto, int i) -> Ids {
+    Ids r = {0, -1.f, 0.f};
+    if (lane < WARPS && i < x.n && (x.sp0 + i) * SPAN < upto) {
+      const int id = __ldg(tab + ((x.sp0 + i) >> 1));
+      if (id < 0 || id >= p.c.pages) {
+        atomicOr(status, STATUS_BAD_ARG);
+      } else {
+        r.pid = id;
+        r.sk = __ldg(p.c.k_scale + static_cast<long long>(id) * kv + x.kvh);
+        r.sv = __ldg(p.c.v_scale + static_cast<long long>(id) * kv + x.kvh);
+      }
+    }
+    return r;
+  };
+  // a segment's rows, four dims a lane
+  uint2 qw[ROWS];
+  auto load_q = [&](const Seg& x) {
+    int tok = 0, hd = 0;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      qw[r] = make_uint2(0u, 0u);
+      if (tok < x.tok)
+        qw[r] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + (x.row0 + tok) * p.ld_q +
+                                                     (x.head0 + hd) * 128 + 4 * lane));
+      if (++hd >= x.nh) {
+        hd = 0;
+        ++tok;
+      }
+    }
+  };
+
+  // lane w < WARPS serves computing warp w: spans TURN, TURN + WARPS, .. of a segment, through its ring's slot
+  // SLOT next; its page numbers and scales are read a span ahead
+  int turn = lane, slot = 0;
+  uint32_t phase = 0, use = 0;
+  Seg cur = advance();
+  const int* cur_table = table;
+  int cur_seen = seen;
+  Ids ids = {};
+  if (cur.n) {
+    ids = fetch_ids(cur, cur_table, cur_seen, turn);
+    load_q(cur);
+  }
+  bool ok = true;
+  for (int k = 0;; ++k) {
+    const int b = k & 1;
+    ok = ok && mbar_wait_uniform(&sh.seg_empty[b], ((k >> 1) & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+    if (!ok) cur.n = 0;
+    if (cur.n) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const float2 v01 = unpack16<F16>(qw[r].x), v23 = unpack16<F16>(qw[r].y);
+        const float v[4] = {v01.x, v01.y, v23.x, v23.y};
+        float mx = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          mx = fmaxf(mx, fabsf(v[i]));
+          bad |= !(fabsf(v[i]) < INFINITY);
+        }
+        if (bad) mx = INFINITY;
+        // the bits of floats that are not negative order as integers do
+        mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+        bad = !(mx < INFINITY);
+        const int e = scale_exponent(bad ? 0.f : mx);
+        const float inv = pow2(-e);
+        uint32_t hi = 0, lo = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = v[i] * inv, h = floorf(x + 0.5f);
+          hi |= (static_cast<uint32_t>(static_cast<int>(h)) & 0xffu) << (8 * i);
+          lo |= (static_cast<uint32_t>(min(__float2int_rn((x - h) * 256.f), 127)) & 0xffu) << (8 * i);
+        }
+        sh.q[b][0][r][lane] = hi;
+        sh.q[b][1][r][lane] = lo;
+        if (lane == 0) sh.q_scale[b][r] = bad ? __uint_as_float(0x7fffffffu) : p.scale_log2 * pow2(e);  // not finite: NaN
+      }
+    }
+    if (lane == 0) {
+      sh.seg[b] = cur;
+      sh.part_len = part_len;
+      sh.lead = lead;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.seg_full[b]);
+    if (!cur.n) break;
+    // the next segment's rows and pages are on their way while this one's spans are dealt out
+    const Seg next = advance();
+    const int* next_table = table;
+    const int next_seen = seen;
+    const int after = turn + (cur.n > turn ? (cur.n - turn + WARPS - 1) / WARPS * WARPS : 0) - cur.n;  // TURN then
+    Ids first = {};
+    if (next.n) {
+      first = fetch_ids(next, next_table, next_seen, after);
+      load_q(next);
+    }
+    Ids then = fetch_ids(cur, cur_table, cur_seen, turn + WARPS);
+    bool left = ok && lane < WARPS && turn < cur.n, v = false;
+    uint64_t since = 0;
+    while (__any_sync(0xffffffffu, left)) {
+      const bool ready = left && mbar_test_wait(&sh.empty[lane][slot], phase ^ 1);
+      if (ready) {
+        const int sp = cur.sp0 + turn;
+        if (!v)
+          sh.meta[lane][use & 1] =
+              make_float4(ids.sk, ids.sv, __int_as_float(ids.sk < 0.f ? 0x7ffffff0 - SPAN : sp * SPAN), 0.f);
+        mbar_arrive_expect_tx(&sh.full[lane][slot], SPAN_BYTES);
+        tma_load_3d(ring + (lane * SLOTS + slot) * SPAN_BYTES, v ? tmV : tmK, &sh.full[lane][slot], 0, (sp & 1) * SPAN,
+                    ids.pid * kv + cur.kvh);
+        if (++slot == SLOTS) {
+          slot = 0;
+          phase ^= 1;
+        }
+        if (v) {
+          ++use;
+          turn += WARPS;
+          left = turn < cur.n;
+          ids = then;
+          then = fetch_ids(cur, cur_table, cur_seen, turn + WARPS);
+        }
+        v = !v;
+      }
+      if (__any_sync(0xffffffffu, ready)) {
+        since = 0;
+      } else {  // every ring is full
+        const uint64_t now = globaltimer();
+        if (since == 0) since = now;
+        if (__any_sync(0xffffffffu, *abort_flag != 0 || now - since > EXN_WAIT_NS)) {
+          if (lane == 0 && !*abort_flag) {
+            *abort_flag = 1;
+            atomicOr(status, STATUS_TIMEOUT_ATTN);
+          }
+          __syncwarp();
+          left = false;
+          ok = false;
+        }
+        __nanosleep(32);
+      }
+    }
+    turn = after;
+    cur = next;
+    cur_table = next_table;
+    cur_seen = next_seen;
+    ids = first;
+  }
+}
+
+template <bool F16, int NT>
+__global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
     k_cache_attend(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const CacheAttnArgs p, int hpt, int head_tiles, int tpt, int* status) {
-  using C = AttendCfg<WARPS, NT>;
-  constexpr int ROWS = C::ROWS;
+                   const CacheAttnArgs p, const AttendPlan plan, int* status) {
+  using C = AttendCfg<NT>;
+  constexpr int ROWS = C::ROWS, WARPS = C::WARPS, SLOTS = C::SLOTS, THREADS = WARPS * 32;  // computing threads
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  int* flags = reinterpret_cast<int*>(smem + C::OFF_BAR + WARPS * C::SLOTS * 8);  // found, abort
-  float* join_m = reinterpret_cast<float*>(smem + C::OFF_JOIN);
-  float* join_l = join_m + ROWS;
-  volatile int* abort_flag = flags + 1;
+  float (*part_o)[ROWS][128] = reinterpret_cast<float (*)[ROWS][128]>(smem + C::RING);  // [WARPS]
+  __shared__ __align__(16) AttendShared<NT> sh;
+  volatile int* abort_flag = &sh.abort_word;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gi = lane >> 2, ti = lane & 3;
-  const int ncta = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-  const int kv = p.c.kv_heads, g = p.heads / kv;
-  int item = blockIdx.x / ncta;
-  const int kvh = item % kv;
-  item /= kv;
-  const int ht = item % head_tiles, slot = item / head_tiles;
   if (threadIdx.x == 0) {
-    flags[0] = -1;
-    flags[1] = 0;
-    for (int i = 0; i < WARPS * C::SLOTS; ++i) mbar_init(&full[i], 1);
+    sh.abort_word = 0;
+    for (int i = 0; i < WARPS * SLOTS; ++i) {
+      mbar_init(&sh.full[0][0] + i, 1);
+      mbar_init(&sh.empty[0][0] + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.seg_full[i], 1);
+      mbar_init(&sh.seg_empty[i], WARPS);
+    }
     fence_mbar_init();
   }
+  __syncthreads();
   griddep_wait();
   griddep_launch();
-  __syncthreads();
-  // sequence s owns the row tiles from floor(start_s / tpt) + s on (from start_s when tpt is 1)
-  for (int s = threadIdx.x; s < p.c.nseq; s += WARPS * 32) {
-    const long long a = p.offsets[s], b = p.offsets[s + 1];
-    if (a < 0 || b < a || b > p.rows || p.c.lens[s] < 0) {
-      if (blockIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
-      continue;
-    }
-    const long long first = tpt == 1 ? a : a / tpt + s;
-    if (slot >= first && slot < first + (b - a + tpt - 1) / tpt) flags[0] = s;
+  if (warp == WARPS) {
+    attend_produce<F16, NT>(&tmK, &tmV, p, plan, sh, smem, status);
+    return;
   }
-  __syncthreads();
-  const int seq = flags[0];
-  if (seq < 0) return;  // the whole cluster: every CTA of it has the same slot
-  const int start = p.offsets[seq], count = p.offsets[seq + 1] - start;
-  const int t0 = (slot - (tpt == 1 ? start : start / tpt + seq)) * tpt;  // first token of the tile
-  const int ntok = min(tpt, count - t0);
-  const int delta = p.c.lens[seq] - count;                               // token t is position t + delta
-  const int h0 = ht * hpt, nh = min(hpt, g - h0);                        // its heads kvh g + h0 ..
-  const int nrows = ntok * nh;
-  const int seen = t0 + ntok + delta;  // positions the tile's last row sees
-  int npages = seen > 0 ? (seen + kPage - 1) / kPage : 0;
-  if (npages > p.c.table_ld) {
-    if (threadIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
-    npages = p.c.table_ld;
-  }
-  const int* table = p.c.table + static_cast<long long>(seq) * p.c.table_ld;
-  const int w0 = rank * WARPS + warp, wn = ncta * WARPS;
-  const int mine = npages > w0 ? (npages - w0 + wn - 1) / wn : 0;  // pages w0, w0 + wn, ..
 
-  // Q^T as the MMA's 16 x 8 operand: this thread's query row is gi (+ 8), its dims 32 ti .. + 31;
-  // k-step ks multiplies dims 32 ti + 4 ks .. + 3.  The row's exponent is brought below 2^15.
-  uint32_t qf[NT][16];
-  int qexp[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int row = nt * 8 + gi;
-    uint4 w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (row < nrows) {
-      const int tok = row / nh, hd = row - tok * nh;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
-                                                        (start + t0 + tok) * p.ld_q + (kvh * g + h0 + hd) * 128 + 32 * ti);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = __ldg(src + i);
-    }
-    const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
-    if (F16) {
-      qexp[nt] = 0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) qf[nt][i] = u[i];
-    } else {
-      float mx = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 f = unpack16<false>(u[i]);
-        mx = fmax3(mx, fabsf(f.x), fabsf(f.y));
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;  // floor(log2 mx)
-      qexp[nt] = mx > 0.f && e < 128 ? max(e - 14, -112) : 0;           // 0 as well for an infinity
-      const float f0 = pow2(-qexp[nt]);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float2 f = unpack16<false>(u[i]);
-        qf[nt][i] = pack16<true>(f.x * f0, f.y * f0);
-      }
-    }
-  }
-  // the thread's score columns: query rows nt * 8 + 2 ti + {0, 1}
-  float qs[NT][2];
-  int lim[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int row = nt * 8 + 2 * ti + j;
-      qs[nt][j] = p.scale_log2 * pow2(__shfl_sync(0xffffffffu, qexp[nt], (2 * ti + j) * 4));
-      lim[nt][j] = row < nrows ? t0 + row / nh + delta : -1;
-    }
-
-  // ---- the pages, one at a time; lane 0 keeps up to SLOTS tiles ahead in flight
-  uint8_t* ring = smem + warp * C::SLOTS * PAGE_BYTES;
-  uint64_t* bar = full + warp * C::SLOTS;
-  const uint32_t ring32 = smem_u32(ring);
-  float m[NT][2], l[NT][2], o[NT][8][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
-  }
-  // page ids and scales of the warp's next 32 pages, one a lane
-  int pid = 0;
-  float sk = 0.f, sv = 0.f;
-  auto fetch_ids = [&](int i0) {
-    const int i = i0 + lane;
-    pid = 0;
-    sk = sv = 0.f;
-    if (i < mine) {
-      pid = __ldg(table + w0 + i * wn);
-      if (pid < 0 || pid >= p.c.pages) {  // not a page: its positions are left out (a scale is never negative)
-        atomicOr(status, STATUS_BAD_ARG);
-        pid = 0;
-        sk = -1.f;
-      } else {
-        sk = __ldg(p.c.k_scale + static_cast<long long>(pid) * kv + kvh);
-        sv = __ldg(p.c.v_scale + static_cast<long long>(pid) * kv + kvh);
-      }
-    }
-  };
-  // tile t of the warp: K of its page t / 2 for even t, V for odd t
-  auto issue = [&](int t, int page) {
-    const int sl = t % C::SLOTS;
-    mbar_arrive_expect_tx(&bar[sl], PAGE_BYTES);
-    tma_load_3d(ring + sl * PAGE_BYTES, (t & 1) ? &tmV : &tmK, &bar[sl], 0, 0, page * kv + kvh);
-  };
-  int issued = 0;
-  if (mine > 0) {
-    fetch_ids(0);
-    const int p0 = __shfl_sync(0xffffffffu, pid, 0), p1 = __shfl_sync(0xffffffffu, pid, 1);
-    if (lane == 0) {
-      issue(0, p0);
-      issue(1, p0);
-      if (mine > 1) issue(2, p1);
-    }
-    issued = mine > 1 ? 3 : 2;
-  }
-  int next_pid = 0;  // page i + 1's id, across a change of the 32 in the lanes
+  // ---- the computing warps
+  auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); };
+  const uint32_t ring32 = smem_u32(smem + warp * SLOTS * SPAN_BYTES);
+  uint64_t* const full = sh.full[warp];
+  uint64_t* const empty = sh.empty[warp];
+  int slot = 0;            // of the next tile to read
+  uint32_t phase = 0, use = 0;
+  int turn = warp;         // spans until this warp's next
   bool ok = true;
-  for (int i = 0; i < mine; ++i) {
-    const float skp = __shfl_sync(0xffffffffu, sk, i & 31), svp = __shfl_sync(0xffffffffu, sv, i & 31);
-    const int page_pos = skp < 0.f ? 0x7ffffff0 - kPage : (w0 + i * wn) * kPage;
-    if ((i & 31) == 31 && i + 1 < mine) fetch_ids(i + 1);
-    next_pid = __shfl_sync(0xffffffffu, pid, (i + 1) & 31);
-    ok = ok && mbar_wait_uniform(&bar[(2 * i) % C::SLOTS], static_cast<uint32_t>((2 * i) / C::SLOTS) & 1, abort_flag, status,
-                                 STATUS_TIMEOUT_ATTN);
+  auto step = [&] {
+    __syncwarp();  // the tile is read
+    if (lane == 0) mbar_arrive(&empty[slot]);
+    if (++slot == SLOTS) {
+      slot = 0;
+      phase ^= 1;
+    }
+  };
+
+  for (int k = 0;; ++k) {
+    const int b = k & 1;
+    ok = ok && mbar_wait_uniform(&sh.seg_full[b], (k >> 1) & 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
     if (!ok) break;
-    // S^T, 16 positions at a time
-    float s[NT][4][4];
-    {
-      const uint32_t base = ring32 + (2 * i) % C::SLOTS * PAGE_BYTES;
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[nt][mt][j] = 0.f;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // 16 of the thread's 32 dims: chunk 2 ti + half of its rows
-          uint32_t a[4], b[4];
-          const uint32_t off = static_cast<uint32_t>((((2 * ti + half) ^ gi) << 4) + (mt * 16 + gi) * 128);
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(base + off) : "memory");
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(b[0]), "=r"(b[1]), "=r"(b[2]), "=r"(b[3]) : "r"(base + off + 1024) : "memory");
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const uint32_t ua = a[ks] ^ 0x80808080u, ub = b[ks] ^ 0x80808080u;
-            const uint32_t fr[4] = {codes_lo(ua), codes_lo(ub), codes_hi(ua), codes_hi(ub)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma16816(s[nt][mt], fr, qf[nt][2 * (half * 4 + ks)], qf[nt][2 * (half * 4 + ks) + 1]);
-          }
-        }
-      }
-    }
-    // K's slot is free (its reads fed the products above): page i + 1's V, or the K after
-    __syncwarp();
-    if (issued < 2 * mine) {
-      // tile 2 i + 3 = V of page i + 1
-      if (lane == 0) issue(2 * i + 3, next_pid);
-      ++issued;
-    }
-    // softmax: one running maximum and sum a query row and warp
-    float corr[NT][2];
-    uint32_t pf[NT][4][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float f = qs[nt][j] * skp;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            float& x = s[nt][mt][2 * hh + j];
-            x = page_pos + mt * 16 + hh * 8 + gi > lim[nt][j] ? -INFINITY : x * f;
-            mx = fmaxf(mx, x);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mn = fmaxf(m[nt][j], mx);
-        const float mu = mn == -INFINITY ? 0.f : mn;
-        corr[nt][j] = fast_exp2(m[nt][j] - mu);
-        m[nt][j] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            float& x = s[nt][mt][2 * hh + j];
-            x = fast_exp2(x - mu);
-            sum += x;
-          }
-        l[nt][j] = l[nt][j] * corr[nt][j] + sum;
-      }
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int hh = 0; hh < 2; ++hh)
-          pf[nt][mt][hh] = transpose8x8(pack16<true>(s[nt][mt][2 * hh], s[nt][mt][2 * hh + 1]));
-    }
-    ok = mbar_wait_uniform(&bar[(2 * i + 1) % C::SLOTS], static_cast<uint32_t>((2 * i + 1) / C::SLOTS) & 1, abort_flag,
-                           status, STATUS_TIMEOUT_ATTN);
-    if (!ok) break;
-    // O^T: dims 16 gi + 2 i, + 1 in the rows gi, gi + 8 of product i
-    float acc[NT][8][4];
+    const int n = sh.seg[b].n, nh = sh.seg[b].nh, nrows = sh.seg[b].tok * nh, pos0 = sh.seg[b].pos0;
+    if (n == 0) break;
+    // Q^T as the MMA's 32 x 8 operand, hi and lo: this thread's query row is gi (+ 8), its dims 32 ti .. + 31;
+    // k-step ks multiplies dims 32 ti + 8 ks .. + 7 (which dims sit where is free as long as q and K agree)
+    uint32_t qf[NT][2][8];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
+      for (int z = 0; z < 2; ++z)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[nt][q][j] = 0.f;
-    {
-      const uint32_t base = ring32 + (2 * i + 1) % C::SLOTS * PAGE_BYTES;
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        uint32_t w[4][4];  // positions 2 ti, 2 ti + 1, 2 ti + 8, 2 ti + 9 of the 16, dims 16 gi .. + 15
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 2 * ti + (r & 1) + (r >> 1) * 8;
-          const uint32_t off = static_cast<uint32_t>(((gi ^ (row & 7)) << 4) + (mt * 16 + row) * 128);
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(w[r][0]), "=r"(w[r][1]), "=r"(w[r][2]), "=r"(w[r][3])
-                       : "r"(base + off)
-                       : "memory");
+        for (int i = 0; i < 8; i += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(&sh.q[b][z][nt * 8 + gi][8 * ti + i]);
+          qf[nt][z][i] = x.x;
+          qf[nt][z][i + 1] = x.y;
+          qf[nt][z][i + 2] = x.z;
+          qf[nt][z][i + 3] = x.w;
         }
+    // the thread's score columns: query rows nt * 8 + 2 ti + {0, 1}
+    float qs[NT][2];
+    int lim[NT][2];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const uint32_t sel = (q & 1) ? 0x7362 : 0x5140;
-          const uint32_t x = __byte_perm(w[0][q >> 1], w[1][q >> 1], sel) ^ 0x80808080u;
-          const uint32_t y = __byte_perm(w[2][q >> 1], w[3][q >> 1], sel) ^ 0x80808080u;
-          const uint32_t fr[4] = {codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y)};
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][q], fr, pf[nt][mt][0], pf[nt][mt][1]);
-        }
+      for (int j = 0; j < 2; ++j) {
+        const int row = nt * 8 + 2 * ti + j;
+        qs[nt][j] = sh.q_scale[b][row];
+        lim[nt][j] = row < nrows ? pos0 + row / nh : -1;
       }
-    }
-    __syncwarp();
-    if (issued < 2 * mine) {  // V's slot is free: tile 2 i + 4 = K of page i + 2
-      const int np = __shfl_sync(0xffffffffu, pid, (i + 2) & 31);
-      int id = np;
-      if (((i + 2) & 31) == 0) id = __ldg(table + w0 + (i + 2) * wn);  // the lanes still hold the 32 before
-      if (id < 0 || id >= p.c.pages) id = 0;
-      if (lane == 0) issue(2 * i + 4, id);
-      ++issued;
-    }
+
+    float m[NT][2], l[NT][2], o[NT][8][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      // a page that the row does not see at all adds nothing, whatever its scale
-      const float sv0 = page_pos > lim[nt][0] ? 0.f : svp, sv1 = page_pos > lim[nt][1] ? 0.f : svp;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o[nt][q][j] = o[nt][q][j] * corr[nt][j & 1] + ((j & 1) ? sv1 : sv0) * acc[nt][q][j];
+        for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
     }
-  }
-  if (!ok && lane == 0) {  // the copies in flight land before the ring is used again
-    volatile int no_abort = 0;
-    for (int t = issued - C::SLOTS < 0 ? 0 : issued - C::SLOTS; t < issued; ++t)
-      mbar_wait(&bar[t % C::SLOTS], static_cast<uint32_t>(t / C::SLOTS) & 1, &no_abort, nullptr, 0);
-  }
-
-  // ---- join: the warps' parts through shared memory (over the ring), then the CTAs' through the
-  // cluster's.  o = sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w in a fixed order.
-  __syncthreads();
-  float* part_o = reinterpret_cast<float*>(smem);                                // [WARPS][ROWS][128]
-  float* part_m = part_o + WARPS * ROWS * 128;                                   // [WARPS][ROWS]
-  float* part_l = part_m + WARPS * ROWS;
-  float* cta_o = part_l + WARPS * ROWS;                                          // [ROWS][128]
-  static_assert((WARPS * ROWS * 130 + ROWS * 128) * 4 <= C::RING, "the join fits the ring");
+    // V's unit: o is in multiples of UNIT; codes of a page of scale sv are multiplied by sv / UNIT while
+    // that is an exact fp16 factor (2^-24 .. 2^5 of codes up to 127), else the unit changes
+    float unit = 0.f, vscale = 0.f;
+    __half2 vr = __half2half2(__ushort_as_half(0)), vb = vr;
+    for (; turn < n; turn += WARPS) {
+      ok = mbar_wait_uniform(&full[slot], phase, abort_flag, status, STATUS_TIMEOUT_ATTN);
+      if (!ok) break;
+      const float4 meta = sh.meta[warp][use & 1];
+      ++use;
+      const float skp = meta.x, svp = meta.y;
+      const int pos = __float_as_int(meta.z);
+      // S^T, 16 positions at a time
+      int si[NT][2][2][4];
+      {
+        const uint32_t at = ring32 + slot * SPAN_BYTES + gi * 128;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+        for (int half = 0; half < 2; ++half) {  // 16 of the thread's 32 dims: chunk 2 ti + half of its rows gi, gi + 8 of 16
+          uint4 kc[2][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float sum = l[nt][j];
-      sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-      const int row = nt * 8 + 2 * ti + j;
-      if (gi == 0) {
-        part_m[warp * ROWS + row] = m[nt][j];
-        part_l[warp * ROWS + row] = sum;
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) kc[mt][r] = ld_shared_v4(at + (((2 * ti + half) ^ gi) << 4) + mt * 2048 + r * 1024);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const uint4 x = kc[mt][0], y = kc[mt][1];
+                const uint32_t (&q)[8] = qf[nt][z];
+                if (half == 0) mma16832_first(si[nt][mt][z], x.x, y.x, x.y, y.y, q[0], q[1]);
+                else mma16832(si[nt][mt][z], x.x, y.x, x.y, y.y, q[4], q[5]);
+              }
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int z = 0; z < 2; ++z)
+                mma16832(si[nt][mt][z], kc[mt][0].z, kc[mt][1].z, kc[mt][0].w, kc[mt][1].w, qf[nt][z][4 * half + 2],
+                         qf[nt][z][4 * half + 3]);
+        }
       }
-      float4* dst = reinterpret_cast<float4*>(part_o + (warp * ROWS + row) * 128 + 16 * gi);
+      step();
+      // softmax: one running maximum and sum a query row and warp
+      const bool masked = pos + SPAN - 1 > pos0;  // past the last position that every row sees
+      uint32_t pf[NT][2][2];
+      float s[NT][2][4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        dst[q] = make_float4(o[nt][2 * q][j], o[nt][2 * q][j + 2], o[nt][2 * q + 1][j], o[nt][2 * q + 1][j + 2]);
+      for (int nt = 0; nt < NT; ++nt) {
+        float alpha[2];
+        bool need = false;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float sc = qs[nt][j] * skp, sc_lo = sc * 0x1p-8f;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              float& x = s[nt][mt][2 * hh + j];
+              x = fmaf(__int_as_float(si[nt][mt][0][2 * hh + j]) - 12582912.f, sc,
+                       (__int_as_float(si[nt][mt][1][2 * hh + j]) - 12582912.f) * sc_lo);
+              if (masked && pos + mt * 16 + hh * 8 + gi > lim[nt][j]) x = -INFINITY;
+            }
+          float mx = fmaxf(fmax3(s[nt][0][j], s[nt][0][2 + j], s[nt][1][j]), s[nt][1][2 + j]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const bool grow = mx > m[nt][j] + 8.f;
+          alpha[j] = grow ? fast_exp2(m[nt][j] - mx) : 1.f;
+          m[nt][j] = grow ? mx : m[nt][j];
+          need |= grow;
+        }
+        if (__any_sync(0xffffffffu, need)) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) l[nt][j] *= alpha[j];
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[nt][q][j] *= alpha[j & 1];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];  // nothing seen yet: every P is 2^-inf = 0
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+              float& x = s[nt][mt][2 * hh + j];
+              x = fast_exp2(x - mu);
+              l[nt][j] += x;
+            }
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+            pf[nt][mt][hh] = transpose8x8(pack16<true>(s[nt][mt][2 * hh], s[nt][mt][2 * hh + 1]));
+      }
+      if (svp != vscale) {  // the same for the whole warp
+        vscale = svp;
+        float r = svp / unit;  // a ratio of powers of two
+        if (svp != svp) {      // a page of scale NaN: the rows that see a position of it are NaN
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (pos <= lim[nt][j & 1]) o[nt][q][j] = svp;
+          r = 0.f;
+          vscale = 0.f;  // for the next page of its kind
+        } else if (svp == 0.f) {
+          r = 0.f;
+        } else if (!(r >= 0x1p-24f && r <= 32.f)) {
+          float big = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(o[nt][q][j]));
+#pragma unroll
+          for (int x = 16; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+          const float change = unit / svp;
+          if (big > 0.f && big * change > 0x1p100f) {
+            r = 0.f;  // 2^-60 of what the sums hold: it adds nothing to them
+            vscale = 0.f;
+          } else {
+            if (big > 0.f)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) o[nt][q][j] *= change;
+            unit = svp;
+            r = 1.f;
+          }
+        }
+        vr = __float2half2_rn(r);
+        vb = __float2half2_rn(-1152.f * r);
+      }
+      ok = mbar_wait_uniform(&full[slot], phase, abort_flag, status, STATUS_TIMEOUT_ATTN);
+      if (!ok) break;
+      // O^T: dims 16 q + 2 gi, + 1 in the rows gi, gi + 8 of product q; a matrix is 8 positions by 16 codes
+      {
+        const int row = lane & 15;  // of 16 positions; lanes 16 .. 31 take the next 16 codes of the same rows
+        const uint32_t at = ring32 + slot * SPAN_BYTES + row * 128;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t w[4][4];
+#pragma unroll
+          for (int q = 0; q < 8; q += 2)
+            ldmatrix_trans(w[q >> 1], at + mt * 2048 + (((q + (lane >> 4)) ^ (row & 7)) << 4));
+#pragma unroll
+          for (int q = 0; q < 8; q += 2)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t x = w[q >> 1][2 * z] ^ 0x80808080u, y = w[q >> 1][2 * z + 1] ^ 0x80808080u;
+              const uint32_t fr[4] = {v_pair(x, EVEN, vr, vb), v_pair(x, ODD, vr, vb), v_pair(y, EVEN, vr, vb),
+                                      v_pair(y, ODD, vr, vb)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][q + z], fr, pf[nt][mt][0], pf[nt][mt][1]);
+            }
+        }
+      }
+      step();
     }
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < ROWS * 32; idx += WARPS * 32) {
-    const int row = idx >> 5;
-    float mx = -INFINITY;
+    if (!ok) break;
+    turn -= n;
+
+    // ---- join the warps: o = sum_w 2^(m_w - M) o_w, l likewise, in a fixed order
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, part_m[w * ROWS + row]);
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float f = fast_exp2(part_m[w * ROWS + row] - mu);
-      const float4 x = reinterpret_cast<const float4*>(part_o + (w * ROWS + row) * 128)[idx & 31];
-      sum += f * part_l[w * ROWS + row];
-      a.x += f * x.x;
-      a.y += f * x.y;
-      a.z += f * x.z;
-      a.w += f * x.w;
+      for (int j = 0; j < 2; ++j) {
+        float t = l[nt][j];
+        t += __shfl_xor_sync(0xffffffffu, t, 4);
+        t += __shfl_xor_sync(0xffffffffu, t, 8);
+        t += __shfl_xor_sync(0xffffffffu, t, 16);
+        const int row = nt * 8 + 2 * ti + j;
+        if (gi == 0) {
+          sh.m[warp][row] = m[nt][j];
+          sh.l[warp][row] = t;
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          *reinterpret_cast<float2*>(&part_o[warp][row][16 * q + 2 * gi]) =
+              make_float2(o[nt][q][j] * unit, o[nt][q][j + 2] * unit);
+      }
+    const Seg seg = sh.seg[b];
+    const int part_len = sh.part_len, lead = sh.lead;
+    barrier();
+    if (lane == 0) mbar_arrive(&sh.seg_empty[b]);
+    const bool whole = n == seg.spans;
+    // a row's four values at 4 (x & 31), normalised and stored
+    auto store = [&](int row, int x, float4 a, float t) {
+      const float inv = t == 0.f ? 0.f : 1.f / t;  // a row that sees no position is 0
+      const int tok = row / nh, hd = row - tok * nh;
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) + (seg.row0 + tok) * p.ld_out + (seg.head0 + hd) * 128 +
+                                (x & 31) * 4) = make_uint2(pack16<F16>(a.x * inv, a.y * inv), pack16<F16>(a.z * inv, a.w * inv));
+    };
+    const int mine = 2 * blockIdx.x + (seg.sp0 ? 0 : 1);
+    for (int x = threadIdx.x; x < nrows * 32; x += THREADS) {
+      const int row = x >> 5;
+      float mx = sh.m[0][row];
+#pragma unroll
+      for (int w = 1; w < WARPS; ++w) mx = fmaxf(mx, sh.m[w][row]);
+      const float mu = mx == -INFINITY ? 0.f : mx;
+      float t = 0.f;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float c = fast_exp2(sh.m[w][row] - mu);
+        const float4 y = reinterpret_cast<const float4*>(part_o[w][row])[x & 31];
+        t += c * sh.l[w][row];
+        a.x += c * y.x;
+        a.y += c * y.y;
+        a.z += c * y.z;
+        a.w += c * y.w;
+      }
+      if (whole) {
+        store(row, x, a, t);
+      } else {
+        float* dst = plan.part + (static_cast<long long>(mine) * ROWS + row) * 132;
+        *reinterpret_cast<float4*>(dst + (x & 31) * 4) = a;
+        if ((x & 31) == 0) *reinterpret_cast<float2*>(dst + 128) = make_float2(mx, t);
+      }
     }
-    reinterpret_cast<float4*>(cta_o + row * 128)[idx & 31] = a;
-    if ((idx & 31) == 0) {
-      join_m[row] = mx;
-      join_l[row] = sum;
+    barrier();  // the join's memory is free, the part is written
+    if (whole) continue;
+
+    // ---- an item that several CTAs share: the last one to get here joins its parts
+    const unsigned first = seg.item + lead;
+    const int c0 = static_cast<int>(first / static_cast<unsigned>(part_len));
+    const int parts = static_cast<int>((first + seg.spans - 1) / static_cast<unsigned>(part_len)) - c0 + 1;
+    auto part_of = [&](int i) { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
+    if (threadIdx.x == 0) {
+      fence_acq_rel();  // after this part's stores (the block's, by the barrier above)
+      sh.taken = count_part(plan.count + c0, plan.tag) + 1 == parts;
+      if (sh.taken) {
+        fence_acq_rel();  // the others' parts are read after their counts
+        plan.count[c0] = 0;
+      }
+    }
+    barrier();
+    if (sh.taken) {
+      // each part's weight 2^(m - M) and each row's sum (in the join's memory), GROUP threads a row
+      constexpr int GROUP = THREADS / ROWS >= 16 ? 16 : 8;
+      static_assert(GROUP * ROWS <= THREADS && GROUP * ROWS % 32 == 0, "whole warps");
+      float* weight = &part_o[0][0][0];
+      float* part_sum = weight + plan.ctas * ROWS;  // an item has at most CTAS parts: room for both (attend_plan)
+      if (threadIdx.x < GROUP * ROWS) {
+        const int row = threadIdx.x / GROUP, sub = threadIdx.x % GROUP;
+        float mx = -INFINITY, t = 0.f;
+        if (row < nrows)
+          for (int i = sub; i < parts; i += GROUP) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(
+                plan.part + (static_cast<long long>(part_of(i)) * ROWS + row) * 132 + 128));
+            weight[i * ROWS + row] = ml.x;
+            part_sum[i * ROWS + row] = ml.y;
+            mx = fmaxf(mx, ml.x);
+          }
+#pragma unroll
+        for (int x = GROUP / 2; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+        const float mu = mx == -INFINITY ? 0.f : mx;
+        if (row < nrows)
+          for (int i = sub; i < parts; i += GROUP) {
+            const float c = fast_exp2(weight[i * ROWS + row] - mu);
+            weight[i * ROWS + row] = c;
+            t += c * part_sum[i * ROWS + row];
+          }
+#pragma unroll
+        for (int x = GROUP / 2; x > 0; x >>= 1) t += __shfl_xor_sync(0xffffffffu, t, x);
+        if (sub == 0) sh.l[0][row] = t;
+      }
+      barrier();
+      for (int x = threadIdx.x; x < nrows * 32; x += THREADS) {
+        const int row = x >> 5;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i0 = 0; i0 < parts; i0 += 8) {  // eight loads at a time
+          float4 y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i0 + i < parts)
+              y[i] = __ldcg(reinterpret_cast<const float4*>(
+                                plan.part + (static_cast<long long>(part_of(i0 + i)) * ROWS + row) * 132) + (x & 31));
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i0 + i < parts) {
+              const float c = weight[(i0 + i) * ROWS + row];
+              a.x += c * y[i].x;
+              a.y += c * y[i].y;
+              a.z += c * y[i].z;
+              a.w += c * y[i].w;
+            }
+        }
+        store(row, x, a, sh.l[0][row]);
+      }
+      barrier();  // the join's memory is free again
     }
   }
-  if (ncta > 1)
-    cluster_sync();
-  else
-    __syncthreads();
-  for (int idx = rank * WARPS * 32 + threadIdx.x; idx < nrows * 32; idx += ncta * WARPS * 32) {
-    const int row = idx >> 5;
-    float mx = -INFINITY;
-    for (int c = 0; c < ncta; ++c) mx = fmaxf(mx, ld_cluster_f(mapa_shared(join_m + row, c)));
-    const float mu = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < ncta; ++c) {
-      const float f = fast_exp2(ld_cluster_f(mapa_shared(join_m + row, c)) - mu);
-      const float4 x = ld_cluster_f4(mapa_shared(cta_o + row * 128 + (idx & 31) * 4, c));
-      sum += f * ld_cluster_f(mapa_shared(join_l + row, c));
-      a.x += f * x.x;
-      a.y += f * x.y;
-      a.z += f * x.z;
-      a.w += f * x.w;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no position is 0
-    const int tok = row / nh, hd = row - tok * nh;
-    uint16_t* dst = static_cast<uint16_t*>(p.out) + (start + t0 + tok) * p.ld_out + (kvh * g + h0 + hd) * 128 +
-                    (idx & 31) * 4;
-    *reinterpret_cast<uint2*>(dst) =
-        make_uint2(pack16<F16>(a.x * inv, a.y * inv), pack16<F16>(a.z * inv, a.w * inv));
+  if (!ok) {  // the copies in flight to this warp's ring land before the CTA leaves
+    volatile int no_abort = 0;
+    for (int i = 0; i < SLOTS; ++i) mbar_wait(&full[i], phase ^ (i < slot ? 1u : 0u), &no_abort, nullptr, 0, 100000000ull);
   }
-  if (ncta > 1) cluster_sync();  // no CTA leaves while another reads its part
 }
 
-template <bool F16, int WARPS, int NT>
-cudaError_t prepare_attend() {
-  cudaError_t e = cudaFuncSetAttribute(k_cache_attend<F16, WARPS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       AttendCfg<WARPS, NT>::SMEM);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(k_cache_attend<F16, WARPS, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  return e;
-}
-
-template <bool F16, int WARPS, int NT>
-cudaError_t launch_attend(const CacheAttnArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, long long items,
-                          int ncta, int hpt, int head_tiles, int tpt, int* d_status, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * ncta));
-  cfg.blockDim = dim3(WARPS * 32);
-  cfg.dynamicSmemBytes = AttendCfg<WARPS, NT>::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = ncta;
-  at[1].val.clusterDim.y = 1;
-  at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, k_cache_attend<F16, WARPS, NT>, tk, tv, a, hpt, head_tiles, tpt, d_status);
+// A number that no other launch of this process has and that is no likely memory content
+unsigned long long launch_tag() {
+  static std::atomic<unsigned long long> next{std::random_device{}() * 0x9e3779b97f4a7c15ull};
+  unsigned long long t;
+  do t = next.fetch_add(0x9e3779b97f4a7c15ull) << 16;  // an odd step: every 48-bit number once
+  while (t == 0);                                      // 0: no launch's
+  return t;
 }
 
 }  // namespace
@@ -773,10 +1146,11 @@ static int dense_launch(const CacheArgs& c, int f16, void* k, void* v, int* d_st
 }
 
 int cache_prepare() {
-  cudaError_t e = prepare_attend<false, 4, 1>();
-  if (e == cudaSuccess) e = prepare_attend<true, 4, 1>();
-  if (e == cudaSuccess) e = prepare_attend<false, 4, 2>();
-  if (e == cudaSuccess) e = prepare_attend<true, 4, 2>();
+  cudaError_t e = cudaSuccess;
+  for (auto* k : {k_cache_attend<false, 1>, k_cache_attend<true, 1>})
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, AttendCfg<1>::SMEM);
+  for (auto* k : {k_cache_attend<false, 2>, k_cache_attend<true, 2>})
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, AttendCfg<2>::SMEM);
   return static_cast<int>(e);
 }
 
@@ -790,45 +1164,55 @@ static bool dense_path(const CacheArgs& c, int heads, long long rows) {
 }
 static long long dense_rows(const CacheArgs& c) { return static_cast<long long>(c.nseq) * c.table_ld * kPage; }
 
-size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows) {
-  return dense_path(c, heads, rows) ? static_cast<size_t>(dense_rows(c)) * c.kv_heads * 128 * 2 * 2 : 0;
+// the cut of the direct path's work: 8 or 16 query rows a tile, 16 when the sequences' rows (on average)
+// need more than 8; a wave of CTAs
+static AttendPlan attend_plan(const CacheArgs& c, int heads, long long rows, int sms, void* ws) {
+  AttendPlan p;
+  const int g = heads / c.kv_heads;
+  const long long per = (rows + c.nseq - 1) / c.nseq;  // new tokens a sequence
+  const int nt = per * g > 8 ? 2 : 1;
+  p.nt = nt;
+  p.hpt = g < 8 * nt ? g : 8 * nt;
+  p.head_tiles = (g + p.hpt - 1) / p.hpt;
+  const int room = 8 * nt / p.hpt;
+  p.tpt = per < room ? static_cast<int>(per) : room;
+  // a wave, but no more CTAs than the join's memory has room for an item's parts (two floats a row and part)
+  const int wave = sms * (nt == 1 ? AttendCfg<1>::CTAS : AttendCfg<2>::CTAS);
+  const int room_for = (nt == 1 ? AttendCfg<1>::JOIN : AttendCfg<2>::JOIN) / (8 * nt * 8);
+  p.ctas = wave < room_for ? wave : room_for;
+  p.tag = 0;
+  p.part = static_cast<float*>(ws);
+  p.count = reinterpret_cast<unsigned long long*>(p.part + 2ll * p.ctas * 8 * nt * 132);
+  return p;
+}
+size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows, int sms) {
+  if (dense_path(c, heads, rows)) return static_cast<size_t>(dense_rows(c)) * c.kv_heads * 128 * 2 * 2;
+  const AttendPlan p = attend_plan(c, heads, rows, sms, nullptr);
+  return static_cast<size_t>(p.ctas) * (2 * 16 * 132 * 4 + 8);
 }
 
-static int attend_launch(const CacheAttnArgs& a, int sms, int* d_status, cudaStream_t st) {
-  const CacheArgs& c = a.c;
-  const int g = a.heads / c.kv_heads;
+static int attend_launch(const CacheAttnArgs& a, void* ws, int sms, int* d_status, cudaStream_t st) {
+  AttendPlan p = attend_plan(a.c, a.heads, a.rows, sms, ws);
+  p.tag = launch_tag();
+  const bool one = p.nt == 1;
   CUtensorMap tk, tv;
-  const uint64_t d[3] = {128, kPage, static_cast<uint64_t>(c.pages) * c.kv_heads};
+  const uint64_t d[3] = {128, kPage, static_cast<uint64_t>(a.c.pages) * a.c.kv_heads};
   const uint64_t s[2] = {128, PAGE_BYTES};
-  const uint32_t b[3] = {128, kPage, 1};
-  if (make_tmap(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.k, 3, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B) ||
-      make_tmap(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.v, 3, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B))
+  const uint32_t b[3] = {128, SPAN, 1};
+  if (make_tmap(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.c.k, 3, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      make_tmap(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.c.v, 3, d, s, b, CU_TENSOR_MAP_SWIZZLE_128B))
     return -4;
-  // 8 or 16 query rows a tile: 16 when the sequences' rows (on average) need more than 8
-  const long long per = (a.rows + c.nseq - 1) / c.nseq;  // new tokens a sequence
-  const int nt = per * g > 8 ? 2 : 1;
-  const int hpt = g < 8 * nt ? g : 8 * nt, head_tiles = (g + hpt - 1) / hpt;
-  const int room = 8 * nt / hpt;
-  const int tpt = per < room ? static_cast<int>(per) : room;
-  const long long items = (a.rows / tpt + (tpt == 1 ? 0 : c.nseq)) * head_tiles * c.kv_heads;
-  // CTAs a cluster: as many as fill the SMs twice over, while each warp keeps a page to itself
-  int ncta = 1;
-  while (ncta < MAX_CLUSTER && items * ncta * 2 <= 2ll * sms && ncta * 4 < c.table_ld) ncta *= 2;
-  if (items * ncta > 0x7fffffffll) return -1;
-  cudaError_t e;
-  if (a.f16)
-    e = nt == 1 ? launch_attend<true, 4, 1>(a, tk, tv, items, ncta, hpt, head_tiles, tpt, d_status, st)
-                : launch_attend<true, 4, 2>(a, tk, tv, items, ncta, hpt, head_tiles, tpt, d_status, st);
-  else
-    e = nt == 1 ? launch_attend<false, 4, 1>(a, tk, tv, items, ncta, hpt, head_tiles, tpt, d_status, st)
-                : launch_attend<false, 4, 2>(a, tk, tv, items, ncta, hpt, head_tiles, tpt, d_status, st);
-  return static_cast<int>(e);
+  const int threads = one ? AttendCfg<1>::THREADS : AttendCfg<2>::THREADS, smem = one ? AttendCfg<1>::SMEM : AttendCfg<2>::SMEM;
+  return static_cast<int>(launch_pdl(one ? (a.f16 ? k_cache_attend<true, 1> : k_cache_attend<false, 1>)
+                                         : (a.f16 ? k_cache_attend<true, 2> : k_cache_attend<false, 2>),
+                                     dim3(p.ctas), dim3(threads), smem, st, tk, tv, a, p, d_status));
 }
 
 int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, int* d_status, cudaStream_t st) {
   const CacheArgs& c = a.c;
-  if (!dense_path(c, a.heads, a.rows)) return attend_launch(a, sms, d_status, st);
-  if (ws_bytes < cache_attention_workspace(c, a.heads, a.rows) || dense_rows(c) > 0x7fffffffll) return -1;
+  if (ws_bytes < cache_attention_workspace(c, a.heads, a.rows, sms)) return -1;
+  if (!dense_path(c, a.heads, a.rows)) return attend_launch(a, ws, sms, d_status, st);
+  if (dense_rows(c) > 0x7fffffffll) return -1;
   uint16_t* k = static_cast<uint16_t*>(ws);
   uint16_t* v = k + static_cast<size_t>(dense_rows(c)) * c.kv_heads * 128;
   const int r = dense_launch(c, a.f16, k, v, d_status, st);

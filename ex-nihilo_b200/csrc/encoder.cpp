@@ -888,7 +888,7 @@ int run_sequences(exn_enc* e, const char* fn, exn_enc_cache* cache, const int32_
   ps.lens = e->seqs + nseq + 1;
   ps.cache = cache;
   if (cache) {
-    const size_t need = cache_attention_workspace(cache_args(cache, 0, nullptr), e->cfg.heads, n);
+    const size_t need = cache_attention_workspace(cache_args(cache, 0, nullptr), e->cfg.heads, n, e->sms);
     if (need > e->attn_ws_cap) {
       if (e->attn_ws) cudaFree(e->attn_ws);
       e->attn_ws = nullptr;

@@ -184,7 +184,7 @@ struct CacheAttnArgs {
 };
 // WS: cache_attention_workspace's bytes, 16-byte aligned.  0, -1 (size), -4 (tensor map) or a cudaError_t.
 int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, int* d_status, cudaStream_t st);
-size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows);
+size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows, int sms);
 int cache_prepare();
 
 // C = A . (q d)^T with the weights as Q8_0 (gemm_q8.cu): QS int8 [N][K], DK the fp16 scales laid out

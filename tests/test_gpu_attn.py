@@ -284,7 +284,7 @@ class Cache:
         att.cache_attend(self.c, q.data_ptr(), out.data_ptr(), o.data_ptr(), q.shape[0], heads, dtype=GGML[t],
                          ld_q=q.stride(0), ld_out=out.stride(0), workspace=w.data_ptr(), workspace_bytes=n, stream=stream)
         att.sync(stream)
-        self.dense = n > 0
+        self.dense = n == self.c.nseq * self.c.table_ld * 64 * self.kv * D * 2 * 2  # keys and values in 16 bits
         return out
 
     def check_attend(self, out, counts, q, heads, t):
@@ -390,6 +390,18 @@ def test_cache_attend_long(att, heads, kv_heads):
     out = c.attend(att, counts, q, heads, "bf16")
     c.check_attend(out, counts, q, heads, "bf16")
     assert torch.equal(out, c.attend(att, counts, q, heads, "bf16"))
+
+
+@pytest.mark.parametrize("heads,tokens", [(4, 1), (8, 2)])
+def test_cache_attend_one_item_in_hundreds_of_parts(att, heads, tokens):
+    """One key/value head and one long sequence: every CTA of the device has a part of the same item."""
+    c = Cache(1, 800, 1)
+    for i in range(2):
+        c.write(att, [25500], rows(25500, 1, 2 * i, "bf16"), rows(25500, 1, 2 * i + 1, "bf16"), "bf16")
+    q = rows(tokens, heads, 3, "bf16")
+    for _ in range(3):
+        out = c.attend(att, [tokens], q, heads, "bf16")
+        c.check_attend(out, [tokens], q, heads, "bf16")
 
 
 @pytest.mark.parametrize("t", ["bf16", "fp16"])
@@ -569,9 +581,8 @@ def test_bad_device_contents_are_left_out_and_reported(att):
         good = c.attend(att, [1, 1], q[:2], heads, "bf16")  # sequence 1 is written to below
         c.table[0, 1] = wrong
         out = torch.full_like(good, 7.0)
-        att.cache_attend(c.c, q.data_ptr(), out.data_ptr(), one.data_ptr(), 2, heads)
         with pytest.raises(E.ExnError):
-            att.sync()
+            c.attend(att, [1, 1], q[:2], heads, "bf16", out=out)
         assert torch.equal(out[1], good[1])
         for call in (att.cache_write, att.cache_read):
             call(c.c, k.data_ptr(), v.data_ptr(), one.data_ptr(), 2)
