@@ -10,20 +10,22 @@
 // in one pass over the keys: with m the running maximum and l the running sum
 // of 2^(s - m), a larger m scales l and o by 2^(m_old - m_new).
 //
-// One CTA = one key/value head of one sequence and two tiles (a, b) of
-// queries that share every K/V tile.  A tile's 128 rows are 128 / g tokens
-// times the g query heads that read this key/value head, so K and V are
-// loaded once a group, not once a query head, and a short prompt still fills
-// its tiles (a 24-token prompt with g = 4: 96 rows, not 24).  Keys are taken
-// 64 at a time ("units"; loads are 128 keys, two units), each tile only as
-// far as its last row sees.  Roles, as in the single-sequence kernel of
-// attention.cu:
-//   warp 0      TMA: Q_a, Q_b once; K_t, V_t through a ring of 4 slots
-//   warp 1, 2   tcgen05.mma of tile a, b: S_x(u) = Q_x K(u)^T into one of two
-//               TMEM buffers, O_x += P_x(u) V(u) with P_x read from TMEM
-//   warps 3..10 softmax of tile a, then b: one row a thread; P_x(u) written
-//               over S_x(u); O_x rescaled in TMEM only when the row maximum
-//               grows by more than 2^8 (P then stays below 2^8, in range of
+// A work item is one key/value head of one sequence and two tiles (a, b) of queries that share every K/V
+// tile.  A tile's 128 rows are 128 / g tokens times the g query heads that read this key/value head, so K
+// and V are loaded once a group, not once a query head, and a short prompt still fills its tiles (a
+// 24-token prompt with g = 4: 96 rows, not 24).  Keys are taken 64 at a time ("units"; loads are 128 keys,
+// two units), each tile only as far as its last row sees.
+//
+// One CTA an SM takes items one after another, the longest first within a sequence: the grid has a CTA an
+// item, and a running CTA takes over those that have not started (cluster launch control), so the SMs
+// stay evenly loaded without a counter in memory, and barriers, TMEM and tensor maps are set up once.
+// Roles, as in the single-sequence kernel of attention.cu:
+//   warp 0      finds the next item; TMA: Q_a, Q_b once an item; K_t, V_t through a ring of 4 slots, the next
+//               item's behind the last one's
+//   warp 1, 2   tcgen05.mma of tile a, b: S_x(u) = Q_x K(u)^T into one of two TMEM buffers, O_x += P_x(u) V(u)
+//               with P_x read from TMEM; the next item's first S while the last O is stored
+//   warps 3..10 softmax of tile a, then b: one row a thread; P_x(u) written over S_x(u); O_x rescaled in TMEM
+//               only when the row maximum grows by more than 2^8 (P then stays below 2^8, in range of
 //               both 16-bit types)
 // The sums and maxima are fp32; P is rounded to the inputs' 16-bit type (the
 // tensor core's operand), o once at the end.
@@ -50,7 +52,7 @@ constexpr int HALF = TILE * 128;      // bytes of one 64-column swizzled half of
 constexpr int TILE_BYTES = 2 * HALF;  // 32 KB
 constexpr int SLOTS = 4;              // K_0 V_0 K_1 V_1 ... stream through 4 slots
 constexpr int OFF_QA = 0, OFF_QB = TILE_BYTES, OFF_SLOT = 2 * TILE_BYTES, OFF_BAR = (2 + SLOTS) * TILE_BYTES;
-constexpr int PK_SMEM = OFF_BAR + 256 + 1024;
+constexpr int PK_SMEM = OFF_BAR + 512 + 1024;
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 
 // kind::f16 instruction descriptor for 16-bit operands of one type (bf16 or fp16) and fp32 sums
@@ -61,14 +63,50 @@ constexpr uint32_t idesc16(int m, int n, bool b_mn) {
              : idesc_bf16(m, n, false, b_mn);
 }
 
+// A work item; n 0 in both tiles: no row of it sees a key
+struct Item {
+  int q_start, nq, t0, tiles;  // the sequence's first query row and rows, the item's first token and tiles
+  int delta, nu[2], nloads;    // token t sees keys 0 .. t + delta; units of each tile; 128-key loads
+  int kvh;                     // key/value head; -1: no more items
+  int k_start;                 // the sequence's first key row
+};
+
 struct Bars {
-  uint64_t q_full, slot_full[SLOTS], slot_empty[SLOTS];
+  uint64_t q_full[2], q_empty[2], slot_full[SLOTS], slot_empty[SLOTS];
   uint64_t s_full[2][2], p_full[2][2];  // [tile][S buffer]
   uint64_t pv_done[2], o_full[2], done[2];
+  uint64_t item_full[2], item_empty[2], claim_full;
+  uint4 claim;  // cluster launch control's answer
+  Item item[2];
   uint32_t tmem_slot;
   int abort_flag;
-  int seq;  // the item's sequence, -1: none
 };
+
+// Ask for a CTA of the grid that has not started; the answer's 16 bytes land in DST and complete BAR
+__device__ __forceinline__ void claim_request(void* dst, uint64_t* bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(dst)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// the CTA's index that the answer gives us, -1: none was left
+__device__ __forceinline__ int claim_answer(const void* src) {
+  int x, got;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.s32 %1, 1, 0, p;\n\t"
+      "mov.b32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, r;\n\t}"
+      : "=r"(x), "=r"(got)
+      : "r"(smem_u32(src))
+      : "memory");
+  return got ? x : -1;
+}
+
+static_assert(sizeof(Bars) <= 512, "the barriers' room");
 
 template <bool F16>
 __device__ __forceinline__ float2 unpack16(uint32_t w) {
@@ -146,71 +184,26 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = p.heads / p.kv_heads;
-  const int kvh = blockIdx.x % p.kv_heads;
-  // Work item: a pair of tiles.  Sequence s owns the pair slots from floor(start_s / (2 tpt)) + s
-  // on; the distance to the next sequence's first slot is at least ceil(length / (2 tpt)), so the
-  // host knows the count of slots without the lengths.  Later slots first: a sequence's last
-  // tiles see the most keys.
-  const int slot = nslots - 1 - static_cast<int>(blockIdx.x) / p.kv_heads;
-  if (threadIdx.x == 0) bars->seq = -1;
-  griddep_wait();  // the offsets may be the previous kernel's output, as Q, K and V
-  griddep_launch();
-  __syncthreads();
-  for (int s = threadIdx.x; s < p.nseq; s += PK_THREADS) {
-    const long long a = p.q_offsets[s], b = p.q_offsets[s + 1];
-    if (a < 0 || b < a || b > p.rows) {
-      if (blockIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
-      continue;
-    }
-    const long long first = a / (2 * tpt) + s;
-    if (slot >= first && slot < first + (b - a + 2 * tpt - 1) / (2 * tpt)) bars->seq = s;
-  }
-  __syncthreads();
-  const int seq = bars->seq;
-  if (seq < 0) return;
-  const int q_start = p.q_offsets[seq], nq = p.q_offsets[seq + 1] - q_start;
-  long long k_start;
-  int nk;
-  if (p.kv_lens) {
-    k_start = p.kv_stride * seq;
-    nk = p.kv_lens[seq];
-  } else {
-    k_start = p.kv_offsets[seq];
-    nk = p.kv_offsets[seq + 1] - static_cast<int>(k_start);
-  }
-  if (k_start < 0 || nk < 0 || k_start + nk > p.kv_rows) {
-    if (threadIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
-    return;
-  }
-  const int t0 = (slot - (q_start / (2 * tpt) + seq)) * 2 * tpt;  // the pair's first token within the sequence
-  const int tiles = nq - t0 > tpt ? 2 : 1;
-  const int delta = nk - nq;  // token t sees keys 0 .. t + delta
-  int nu[2] = {0, 0};         // units each tile's last row sees
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-    if (x < tiles) {
-      const int seen = min(nq, t0 + (x + 1) * tpt) + delta;
-      nu[x] = seen > 0 ? (seen + UNIT - 1) / UNIT : 0;
-    }
-  const int nunits = max(nu[0], nu[1]);
-  const int nloads = (nunits + 1) / 2;
   uint16_t* const out = static_cast<uint16_t*>(p.out);
-
   if (threadIdx.x == 0) {
-    mbar_init(&bars->q_full, 1);
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(&bars->slot_full[i], 1);
-      mbar_init(&bars->slot_empty[i], tiles);
+      mbar_init(&bars->slot_empty[i], 2);  // free once both tiles' MMAs are done with it
     }
     for (int x = 0; x < 2; ++x) {
       for (int b = 0; b < 2; ++b) {
         mbar_init(&bars->s_full[x][b], 1);
         mbar_init(&bars->p_full[x][b], 4);
       }
+      mbar_init(&bars->q_full[x], 1);
+      mbar_init(&bars->q_empty[x], 1);
       mbar_init(&bars->pv_done[x], 1);
       mbar_init(&bars->o_full[x], 1);
       mbar_init(&bars->done[x], 1);
+      mbar_init(&bars->item_full[x], 1);
+      mbar_init(&bars->item_empty[x], 10);  // the two MMA threads and eight softmax warps
     }
+    mbar_init(&bars->claim_full, 1);
     bars->abort_flag = 0;
     fence_mbar_init();
   }
@@ -223,51 +216,173 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_slot;
   // TMEM columns: S_a buffers [0,64) [64,128), S_b [128,192) [192,256), O_a [256,384), O_b [384,512)
+  griddep_wait();  // the offsets may be the previous kernel's output, as Q, K and V
+  griddep_launch();
+  if (blockIdx.x == 0)  // what is wrong with the offsets is reported once; the items leave it out
+    for (int s = threadIdx.x; s < p.nseq; s += PK_THREADS) {
+      const int a = p.q_offsets[s], b = p.q_offsets[s + 1];
+      if (a < 0 || b < a || b > p.rows) atomicOr(status, STATUS_BAD_ARG);
+    }
+
+  // The waits for the next item are the only ones that do not look at the abort flag, so every role goes through
+  // the same items, with the work left out once a wait has run out, and the tiles' warps stay in step.  The
+  // producer, whose own waits are bounded, ends the list.
+  volatile int no_abort = 0;
+  auto wait_item = [&](uint64_t* bar, uint32_t parity) {  // one thread
+    volatile int none = 0;
+    return mbar_wait(bar, parity, &none, status, STATUS_TIMEOUT_ATTN, 16 * EXN_WAIT_NS);
+  };
 
   if (warp == 0) {
-    if (lane == 0 && nunits > 0) {
+    // ---- the items.  Sequence s owns the pair slots from floor(start_s / (2 tpt)) + s on; the distance to the
+    // next sequence's first slot is at least ceil(length / (2 tpt)), so the host knows the count of slots
+    // without the lengths.  Later slots first: a sequence's last tiles see the most keys.
+    const int pair = 2 * tpt;
+    auto find = [&](int index, Item& x) -> bool {  // by the whole warp; false: nothing at this slot
+      const int sl = nslots - 1 - index / p.kv_heads;
+      int lo = 0, hi = p.nseq;  // the last sequence that owns slots up to SL, 32 probes a step
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, s = lo + lane * step;
+        const bool below = s < hi && p.q_offsets[s] / pair + s <= sl;
+        const unsigned m = __ballot_sync(0xffffffffu, below) | 1u;
+        lo += (31 - __clz(m)) * step;
+        hi = min(hi, lo + step);
+      }
+      const int a = p.q_offsets[lo], b = p.q_offsets[lo + 1];
+      x.t0 = (sl - (a / pair + lo)) * pair;
+      if (a < 0 || b > p.rows || x.t0 < 0 || x.t0 >= b - a) return false;
+      x.q_start = a;
+      x.nq = b - a;
+      long long k_start;
+      int nk;
+      if (p.kv_lens) {
+        k_start = p.kv_stride * lo;
+        nk = p.kv_lens[lo];
+      } else {
+        k_start = p.kv_offsets[lo];
+        nk = p.kv_offsets[lo + 1] - static_cast<int>(k_start);
+      }
+      if (k_start < 0 || nk < 0 || k_start + nk > p.kv_rows) {
+        if (lane == 0) atomicOr(status, STATUS_BAD_ARG);
+        return false;
+      }
+      x.k_start = static_cast<int>(k_start);
+      x.kvh = index % p.kv_heads;
+      x.tiles = x.nq - x.t0 > tpt ? 2 : 1;
+      x.delta = nk - x.nq;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int seen = i < x.tiles ? min(x.nq, x.t0 + (i + 1) * tpt) + x.delta : 0;
+        x.nu[i] = seen > 0 ? (seen + UNIT - 1) / UNIT : 0;
+      }
+      x.nloads = (max(x.nu[0], x.nu[1]) + 1) / 2;
+      return true;
+    };
+    // The next item is asked for late: near the end of the item at hand, and not in the kernel's first
+    // microseconds, when the CTAs that have not started are still finding SMs of their own.
+    uint32_t claims = 0;
+    bool ok = true, asked = false, ended = false;
+    const uint64_t t_start = globaltimer();
+    auto settled = [&] { return __any_sync(0xffffffffu, globaltimer() - t_start > 3000); };
+    auto ask = [&] {
+      if (lane == 0) claim_request(&bars->claim, &bars->claim_full);
+      asked = true;
+    };
+    auto next_item = [&](Item& x) {  // kvh -1: no more
+      x.kvh = -1;
+      while (!ended && ok) {
+        if (!asked) {
+          while (!settled()) __nanosleep(100);
+          ask();
+        }
+        if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->claim_full, claims & 1) : true, 0)) {
+          ok = false;
+          return;
+        }
+        ++claims;
+        asked = false;
+        const int index = claim_answer(&bars->claim);
+        ended = index < 0;
+        fence_proxy_async_smem();  // the answer is read before the next one is written
+        __syncwarp();
+        if (!ended && find(index, x)) return;
+        x.kvh = -1;
+      }
+    };
+    if (lane == 0) {
       tma_prefetch(&tmQ);
       tma_prefetch(&tmK);
       tma_prefetch(&tmV);
-      // a tile of Q: the box (64 dims, g heads, tpt tokens), rows token-major; rows of the tile
-      // past g tpt stay as they are and are never stored
-      mbar_arrive_expect_tx(&bars->q_full, tiles * 2 * g * tpt * 128);
-      for (int x = 0; x < tiles; ++x)
-        for (int hf = 0; hf < 2; ++hf)
-          tma_load_3d(smem + (x ? OFF_QB : OFF_QA) + hf * HALF, &tmQ, &bars->q_full, hf * 64, kvh * g,
-                      q_start + t0 + x * tpt);
-      int issued = 0;
-      for (int t = 0; t < 2 * nloads; ++t) {
-        const int sl = t % SLOTS;
-        const uint32_t use = static_cast<uint32_t>(t / SLOTS);
-        if (!mbar_wait(&bars->slot_empty[sl], (use & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN)) break;
-        mbar_arrive_expect_tx(&bars->slot_full[sl], TILE_BYTES);
-        const CUtensorMap* map = (t & 1) ? &tmV : &tmK;
-        for (int hf = 0; hf < 2; ++hf)
-          tma_load_2d(smem + OFF_SLOT + sl * TILE_BYTES + hf * HALF, map, &bars->slot_full[sl], kvh * 128 + hf * 64,
-                      static_cast<int>(k_start) + (t >> 1) * TILE);
-        issued = t + 1;
+    }
+    Item cur;
+    if (!find(static_cast<int>(blockIdx.x), cur)) next_item(cur);
+    uint32_t q_count[2] = {0, 0}, loads = 0;  // so far
+    for (uint32_t k = 0;; ++k) {
+      const int ib = k & 1;
+      if (*abort_flag) ok = false;
+      if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->item_empty[ib], ((k >> 1) & 1) ^ 1) : true, 0)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) cur.kvh = -1;
+      if (lane == 0) {
+        bars->item[ib] = cur;
+        mbar_arrive(&bars->item_full[ib]);
       }
-      if (*abort_flag) {  // the copies in flight land before the CTA leaves
-        volatile int no_abort = 0;
-        mbar_wait(&bars->q_full, 0, &no_abort, nullptr, 0);
-        for (int t = issued - SLOTS < 0 ? 0 : issued - SLOTS; t < issued; ++t)
-          mbar_wait(&bars->slot_full[t % SLOTS], static_cast<uint32_t>(t / SLOTS) & 1, &no_abort, nullptr, 0);
+      __syncwarp();
+      if (cur.kvh < 0) break;
+      // a tile of Q: the box (64 dims, g heads, tpt tokens), rows token-major; rows of the tile past g tpt stay
+      // as they are and are never stored
+      if (cur.nloads > 0)
+        for (int x = 0; x < cur.tiles; ++x) {
+          ok = ok && mbar_wait_warp(&bars->q_empty[x], (q_count[x] & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&bars->q_full[x], 2 * g * tpt * 128);
+            for (int hf = 0; hf < 2; ++hf)
+              tma_load_3d(smem + (x ? OFF_QB : OFF_QA) + hf * HALF, &tmQ, &bars->q_full[x], hf * 64, cur.kvh * g,
+                          cur.q_start + cur.t0 + x * tpt);
+          }
+          ++q_count[x];
+        }
+      Item next;
+      for (int t = 0; t < 2 * cur.nloads; ++t) {
+        if (t >= 2 * cur.nloads - 8 && !asked && !ended && settled()) ask();
+        if (!ok) continue;
+        const uint32_t sl = loads % SLOTS;
+        ok = mbar_wait_warp(&bars->slot_empty[sl], ((loads / SLOTS) & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+        if (!ok) continue;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->slot_full[sl], TILE_BYTES);
+          const CUtensorMap* map = (t & 1) ? &tmV : &tmK;
+          for (int hf = 0; hf < 2; ++hf)
+            tma_load_2d(smem + OFF_SLOT + sl * TILE_BYTES + hf * HALF, map, &bars->slot_full[sl], cur.kvh * 128 + hf * 64,
+                        cur.k_start + (t >> 1) * TILE);
+        }
+        ++loads;
       }
+      next_item(next);
+      cur = next;
+    }
+    if (!ok && lane == 0) {  // the copies in flight, and an answer, land before the CTA leaves
+      for (int x = 0; x < 2; ++x)
+        if (q_count[x]) mbar_wait(&bars->q_full[x], (q_count[x] - 1) & 1, &no_abort, nullptr, 0);
+      for (uint32_t t = loads < SLOTS ? 0 : loads - SLOTS; t < loads; ++t)
+        mbar_wait(&bars->slot_full[t % SLOTS], (t / SLOTS) & 1, &no_abort, nullptr, 0);
+      if (asked) mbar_wait(&bars->claim_full, claims & 1, &no_abort, nullptr, 0);
     }
   } else if (warp <= 2) {
-    if (lane == 0 && warp - 1 < tiles && nunits > 0) {
+    if (lane == 0) {
       // ---- the MMAs of tile x (descriptors as 32-bit low words over a common high word)
       const int x = warp - 1;
-      const int n = nu[x];
       const uint32_t dhi = static_cast<uint32_t>(sdesc_sw128(0, 16, 1024) >> 32);
       const uint32_t qlo = static_cast<uint32_t>(sdesc_sw128(smem_u32(smem + (x ? OFF_QB : OFF_QA)), 16, 1024));
       const uint32_t klo = static_cast<uint32_t>(sdesc_sw128(smem_u32(smem + OFF_SLOT), 16, 1024));    // K-major
       const uint32_t vlo = static_cast<uint32_t>(sdesc_sw128(smem_u32(smem + OFF_SLOT), HALF, 1024));  // MN-major
       const uint32_t s_tm = tmem + x * 128, o_tm = tmem + 256 + x * 128;
+      uint32_t base = 0, units = 0, q_count = 0;  // loads and this tile's units of the items before
+      auto slot_of = [&](int t) { return (base + t) % SLOTS; };
       auto issue_s = [&](int u) {
-        const uint32_t k = klo + ((((u >> 1) * 2) % SLOTS) * TILE_BYTES + (u & 1) * UNIT * 128) / 16;
-        const uint32_t d = s_tm + (u & 1) * UNIT;
+        const uint32_t k = klo + (slot_of((u >> 1) * 2) * TILE_BYTES + (u & 1) * UNIT * 128) / 16;
+        const uint32_t d = s_tm + ((units + u) & 1) * UNIT;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) {
           const uint32_t o = ((kk >> 2) * HALF + (kk & 3) * 32) / 16;
@@ -275,205 +390,229 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         }
       };
       auto issue_pv = [&](int u) {
-        const uint32_t v = vlo + ((((u >> 1) * 2 + 1) % SLOTS) * TILE_BYTES + (u & 1) * UNIT * 128) / 16;
-        const uint32_t a = s_tm + (u & 1) * UNIT;
+        const uint32_t v = vlo + (slot_of((u >> 1) * 2 + 1) * TILE_BYTES + (u & 1) * UNIT * 128) / 16;
+        const uint32_t a = s_tm + ((units + u) & 1) * UNIT;
 #pragma unroll
         for (int kk = 0; kk < UNIT / 16; ++kk)
           umma_ts_lo(o_tm, a + kk * 8, v + kk * 2048 / 16, dhi, IDESC_PV, (u > 0 || kk) ? 1u : 0u);
       };
       auto wait_load = [&](int t) {
-        return mbar_wait(&bars->slot_full[t % SLOTS], static_cast<uint32_t>(t / SLOTS) & 1, abort_flag, status,
-                         STATUS_TIMEOUT_ATTN);
+        return mbar_wait(&bars->slot_full[slot_of(t)], ((base + t) / SLOTS) & 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
       };
-      bool ok = mbar_wait(&bars->q_full, 0, abort_flag, status, STATUS_TIMEOUT_ATTN);
-      if (ok && n > 0 && (ok = wait_load(0))) {
-        tc_fence_after();
-        for (int u = 0; u < 2 && u < n; ++u) {
-          issue_s(u);
-          umma_commit(&bars->s_full[x][u]);
+      bool ok = true;
+      for (uint32_t k = 0;; ++k) {
+        const int ib = k & 1;
+        if (!wait_item(&bars->item_full[ib], (k >> 1) & 1)) break;
+        const int n = bars->item[ib].nu[x], nloads = bars->item[ib].nloads;
+        const bool has_q = nloads > 0 && x < bars->item[ib].tiles, last = bars->item[ib].kvh < 0;
+        mbar_arrive(&bars->item_empty[ib]);
+        if (last) break;
+        if (has_q) {
+          ok = ok && mbar_wait(&bars->q_full[x], q_count & 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+          ++q_count;
+          if (ok && n == 0) umma_commit(&bars->q_empty[x]);
         }
-        umma_commit(&bars->slot_empty[0]);  // K_0: both its units issued
-      }
-      for (int u = 0; u < n && ok; ++u) {
-        const int b = u & 1;
-        const bool more = u + 2 < n;
-        if (b == 0 && !(ok = wait_load(2 * (u >> 1) + 1))) break;  // V(u)
-        if (!(ok = mbar_wait(&bars->p_full[x][b], static_cast<uint32_t>(u >> 1) & 1, abort_flag, status,
-                             STATUS_TIMEOUT_ATTN)))
-          break;
-        tc_fence_after();
-        issue_pv(u);
-        umma_commit(&bars->pv_done[x]);
-        if (u + 1 == n) umma_commit(&bars->o_full[x]);
-        if (more) {
-          if (b == 0 && !(ok = wait_load(2 * ((u + 2) >> 1)))) break;  // K(u + 2)
-          issue_s(u + 2);
-          umma_commit(&bars->s_full[x][b]);
+        if (ok && n > 0 && (ok = wait_load(0))) {
+          tc_fence_after();
+          for (int u = 0; u < 2 && u < n; ++u) {
+            issue_s(u);
+            umma_commit(&bars->s_full[x][(units + u) & 1]);
+          }
+          umma_commit(&bars->slot_empty[slot_of(0)]);  // K_0: both its units issued
+          if (n <= 2) umma_commit(&bars->q_empty[x]);
         }
-        // this tile's share of freeing the slots whose last reader was just issued
-        if (b == 1 || u + 1 == n) umma_commit(&bars->slot_empty[(2 * (u >> 1) + 1) % SLOTS]);   // V(u)
-        if (more && (b == 1 || u + 3 == n)) umma_commit(&bars->slot_empty[(2 * ((u + 2) >> 1)) % SLOTS]);
-      }
-      // the loads only the other tile reads: this tile's share once each has landed
-      for (int t = 2 * ((n + 1) / 2); t < 2 * nloads && ok; ++t) {
-        if (!(ok = wait_load(t))) break;
-        umma_commit(&bars->slot_empty[t % SLOTS]);
+        for (int u = 0; u < n && ok; ++u) {
+          const int b = (units + u) & 1;
+          const bool more = u + 2 < n;
+          if ((u & 1) == 0 && !(ok = wait_load(2 * (u >> 1) + 1))) break;  // V(u)
+          if (!(ok = mbar_wait(&bars->p_full[x][b], ((units + u) >> 1) & 1, abort_flag, status, STATUS_TIMEOUT_ATTN))) break;
+          tc_fence_after();
+          issue_pv(u);
+          umma_commit(&bars->pv_done[x]);
+          if (u + 1 == n) umma_commit(&bars->o_full[x]);
+          if (more) {
+            if ((u & 1) == 0 && !(ok = wait_load(2 * ((u + 2) >> 1)))) break;  // K(u + 2)
+            issue_s(u + 2);
+            umma_commit(&bars->s_full[x][b]);
+            if (u + 3 == n) umma_commit(&bars->q_empty[x]);
+          }
+          // this tile's share of freeing the slots whose last reader was just issued
+          if ((u & 1) == 1 || u + 1 == n) umma_commit(&bars->slot_empty[slot_of(2 * (u >> 1) + 1)]);   // V(u)
+          if (more && ((u & 1) == 1 || u + 3 == n)) umma_commit(&bars->slot_empty[slot_of(2 * ((u + 2) >> 1))]);
+        }
+        // the loads only the other tile reads: this tile's share once each has landed
+        for (int t = 2 * ((n + 1) / 2); t < 2 * nloads && ok; ++t) {
+          if (!(ok = wait_load(t))) break;
+          umma_commit(&bars->slot_empty[slot_of(t)]);
+        }
+        base += 2 * nloads;
+        units += n;
       }
       umma_commit(&bars->done[x]);  // every MMA queued above has finished before TMEM is released
-      volatile int no_abort = 0;
       mbar_wait(&bars->done[x], 0, &no_abort, nullptr, 0);
     }
-  } else if ((warp - 3) >> 2 < tiles) {
+  } else {
     // ---- softmax: tile x, TMEM lane quarter wq, row r of the tile
     const int x = (warp - 3) >> 2;
-    const int n = nu[x];
     const int wq = warp & 3;
     const int r = wq * 32 + lane;
     const int tok = r / g;
-    const int t = t0 + x * tpt + tok;  // token within the sequence
-    const bool live = tok < tpt && t < nq;
-    const int lim = live ? t + delta : n * UNIT;  // last visible key (< 0: none)
     const uint32_t lane_off = static_cast<uint32_t>(wq * 32) << 16;
     const uint32_t s_addr = tmem + lane_off + x * 128;
     const uint32_t o_addr = tmem + lane_off + 256 + x * 128;
-    float m = -INFINITY, lsum = 0.f;
-    bool ok = true;
     const uint64_t sc2 = f2(p.scale_log2, p.scale_log2);
-    // the two tiles' exponentials take turns on each scheduler (attention.cu); tile a's turns end
-    // with its last unit, which is never after tile b's
+    // the two tiles' exponentials take turns on each scheduler (attention.cu); tile a's turns end with its
+    // last unit, which is never after tile b's
     const uint32_t my_turn = (x ? 5u : 1u) + static_cast<uint32_t>(wq);
     const uint32_t other_turn = (x ? 1u : 5u) + static_cast<uint32_t>(wq);
-    const int turns = tiles == 2 ? nu[0] : 0;
-    if (turns > 0 && x == 1) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");  // tile a goes first
-    for (int u = 0; u < n; ++u) {
-      const int b = u & 1;
-      ok = ok && mbar_wait_uniform(&bars->s_full[x][b], static_cast<uint32_t>(u >> 1) & 1, abort_flag, status,
-                                   STATUS_TIMEOUT_ATTN);
-      float s[UNIT];
-      float nm = 0.f;
-      if (ok) {
-        tc_fence_after();
-        {
-          uint32_t rr[UNIT];
-          tmem_ld64_conv(s_addr + b * UNIT, rr);
+    uint32_t units = 0, o_count = 0;  // of the items before
+    bool ok = true;
+    for (uint32_t k = 0;; ++k) {
+      const int ib = k & 1;
+      if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->item_full[ib], (k >> 1) & 1) : true, 0)) break;
+      const Item& it = bars->item[ib];
+      const int kvh = it.kvh, n = it.nu[x], n_a = it.nu[0], tiles = it.tiles, delta = it.delta, nq = it.nq;
+      const int t = it.t0 + x * tpt + tok, q_start = it.q_start, k_start = it.k_start;  // t: token within the sequence
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->item_empty[ib]);
+      if (kvh < 0) break;
+      const bool live = tok < tpt && t < nq && x < tiles;
+      const int lim = live ? t + delta : n * UNIT;  // last visible key (< 0: none)
+      float m = -INFINITY, lsum = 0.f;
+      const int turns = tiles == 2 ? n_a : 0;
+      if (turns > 0 && x == 1) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");  // tile a goes first
+      for (int u = 0; u < n; ++u) {
+        const int b = (units + u) & 1;
+        ok = ok && mbar_wait_uniform(&bars->s_full[x][b], ((units + u) >> 1) & 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+        float s[UNIT];
+        float nm = 0.f;
+        if (ok) {
+          tc_fence_after();
+          {
+            uint32_t rr[UNIT];
+            tmem_ld64_conv(s_addr + b * UNIT, rr);
 #pragma unroll
-          for (int i = 0; i < UNIT; ++i) s[i] = __uint_as_float(rr[i]);
-        }
-        const int key0 = u * UNIT;
-        if (__any_sync(0xffffffffu, key0 + UNIT - 1 > lim)) {
+            for (int i = 0; i < UNIT; ++i) s[i] = __uint_as_float(rr[i]);
+          }
+          const int key0 = u * UNIT;
+          if (__any_sync(0xffffffffu, key0 + UNIT - 1 > lim)) {
 #pragma unroll
-          for (int c = 0; c < UNIT; ++c)
-            if (key0 + c > lim) s[c] = -INFINITY;
-        }
-        float m8[8];
+            for (int c = 0; c < UNIT; ++c)
+              if (key0 + c > lim) s[c] = -INFINITY;
+          }
+          float m8[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = fmax3(s[i], s[8 + i], s[16 + i]);
+          for (int i = 0; i < 8; ++i) m8[i] = fmax3(s[i], s[8 + i], s[16 + i]);
 #pragma unroll
-        for (int c = 24; c < UNIT - 8; c += 16)
+          for (int c = 24; c < UNIT - 8; c += 16)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) m8[i] = fmax3(m8[i], s[c + i], s[c + 8 + i]);
+            for (int i = 0; i < 8; ++i) m8[i] = fmax3(m8[i], s[c + i], s[c + 8 + i]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(m8[i], s[UNIT - 8 + i]);
-        const float mx = fmaxf(fmax3(m8[0], m8[1], m8[2]), fmax3(fmax3(m8[3], m8[4], m8[5]), m8[6], m8[7]));
-        const float m_new = fmaxf(m, mx * p.scale_log2);
-        const bool need = m_new > m + RESCALE_THRESHOLD;
-        const float alpha = need ? fast_exp2(m - m_new) : 1.f;
-        lsum *= alpha;
-        m = need ? m_new : m;
-        nm = m == -INFINITY ? 0.f : -m;  // nothing seen yet: every P is 2^-inf = 0
-        if (u > 0 && __any_sync(0xffffffffu, need)) {
-          ok = mbar_wait_uniform(&bars->pv_done[x], static_cast<uint32_t>(u - 1) & 1, abort_flag, status,
-                                 STATUS_TIMEOUT_ATTN);
-          if (ok) {
-            tc_fence_after();
+          for (int i = 0; i < 8; ++i) m8[i] = fmaxf(m8[i], s[UNIT - 8 + i]);
+          const float mx = fmaxf(fmax3(m8[0], m8[1], m8[2]), fmax3(fmax3(m8[3], m8[4], m8[5]), m8[6], m8[7]));
+          const float m_new = fmaxf(m, mx * p.scale_log2);
+          const bool need = m_new > m + RESCALE_THRESHOLD;
+          const float alpha = need ? fast_exp2(m - m_new) : 1.f;
+          lsum *= alpha;
+          m = need ? m_new : m;
+          nm = m == -INFINITY ? 0.f : -m;  // nothing seen yet: every P is 2^-inf = 0
+          if (u > 0 && __any_sync(0xffffffffu, need)) {
+            ok = mbar_wait_uniform(&bars->pv_done[x], (units + u - 1) & 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+            if (ok) {
+              tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t ov[32];
-              tmem_ld32(o_addr + c * 32, ov);
+              for (int c = 0; c < 4; ++c) {
+                uint32_t ov[32];
+                tmem_ld32(o_addr + c * 32, ov);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-              tmem_st32(o_addr + c * 32, ov);
+                for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+                tmem_st32(o_addr + c * 32, ov);
+              }
+              tmem_st_wait();
             }
-            tmem_st_wait();
           }
         }
-      }
-      if (u < turns) asm volatile("bar.sync %0, 64;" ::"r"(my_turn) : "memory");
-      uint32_t pk[UNIT / 2];  // P as 16-bit pairs: key 2c and 2c+1 in column c
-      if (ok) {
-        const uint64_t nm2 = f2(nm, nm);
-        uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
+        if (u < turns) asm volatile("bar.sync %0, 64;" ::"r"(my_turn) : "memory");
+        uint32_t pk[UNIT / 2];  // P as 16-bit pairs: key 2c and 2c+1 in column c
+        if (ok) {
+          const uint64_t nm2 = f2(nm, nm);
+          uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-        for (int c8 = 0; c8 < UNIT / 8; ++c8) {
+          for (int c8 = 0; c8 < UNIT / 8; ++c8) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x0, x1;
-            f2_split(ffma2(f2(s[c8 * 8 + 2 * i], s[c8 * 8 + 2 * i + 1]), sc2, nm2), x0, x1);
-            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
-            ps2[i] = fadd2(ps2[i], f2(e0, e1));
-            pk[c8 * 4 + i] = pack16<F16>(e0, e1);
+            for (int i = 0; i < 4; ++i) {
+              float x0, x1;
+              f2_split(ffma2(f2(s[c8 * 8 + 2 * i], s[c8 * 8 + 2 * i + 1]), sc2, nm2), x0, x1);
+              const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+              ps2[i] = fadd2(ps2[i], f2(e0, e1));
+              pk[c8 * 4 + i] = pack16<F16>(e0, e1);
+            }
           }
+          float a0, a1;
+          f2_split(fadd2(fadd2(ps2[0], ps2[1]), fadd2(ps2[2], ps2[3])), a0, a1);
+          lsum += a0 + a1;
         }
-        float a0, a1;
-        f2_split(fadd2(fadd2(ps2[0], ps2[1]), fadd2(ps2[2], ps2[3])), a0, a1);
-        lsum += a0 + a1;
-      }
-      if (u < turns && (x == 0 || u + 1 < turns)) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");
-      if (ok) {
-        tmem_st32_conv(s_addr + b * UNIT, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->p_full[x][b]);
-      }
-    }
-    const int head = kvh * g + r - tok * g;
-    uint16_t* dst = out + static_cast<long long>(q_start + t) * p.ld_out + head * 128;
-    if (n > 0) {
-      if (ok && mbar_wait_uniform(&bars->o_full[x], 0, abort_flag, status, STATUS_TIMEOUT_ATTN)) {
-        tc_fence_after();
-        const bool none = lsum == 0.f;
-        const float inv = none ? 0.f : 1.f / lsum;
-        float finite = 0.f;  // 0 times every output: NaN when one is not finite
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          uint32_t rr[32];
-          tmem_ld32(o_addr + c * 32, rr);
-          float o[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            o[i] = __uint_as_float(rr[i]) * inv;
-            finite = fmaf(o[i], 0.f, finite);
-          }
-          if (live) {
-            uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              d4[i] = make_uint4(pack16<F16>(o[8 * i], o[8 * i + 1]), pack16<F16>(o[8 * i + 2], o[8 * i + 3]),
-                                 pack16<F16>(o[8 * i + 4], o[8 * i + 5]), pack16<F16>(o[8 * i + 6], o[8 * i + 7]));
-          }
-        }
-        __syncwarp();
-        unsigned bad = __ballot_sync(0xffffffffu, live && finite != 0.f);
-        while (bad) {
-          const int src = __ffs(bad) - 1;
-          bad &= bad - 1;
-          const int rt = __shfl_sync(0xffffffffu, t, src), rh = __shfl_sync(0xffffffffu, head, src);
-          const int rl = __shfl_sync(0xffffffffu, lim, src);
-          const long long rows_end = p.kv_rows - k_start;  // rows past the tensor were read as zeros
-          const int last = static_cast<int>(min(static_cast<long long>(n) * UNIT, rows_end)) - 1;
-          const uint16_t* kb = static_cast<const uint16_t*>(p.k) + k_start * p.ld_k + kvh * 128;
-          const uint16_t* vb = static_cast<const uint16_t*>(p.v) + k_start * p.ld_v + kvh * 128;
-          mend_row<F16>(static_cast<const uint16_t*>(p.q) + static_cast<long long>(q_start + rt) * p.ld_q + rh * 128,
-                        kb, p.ld_k, vb, p.ld_v, rl, last, p.scale_log2,
-                        out + static_cast<long long>(q_start + rt) * p.ld_out + rh * 128);
+        if (u < turns && (x == 0 || u + 1 < turns)) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");
+        if (ok) {
+          tmem_st32_conv(s_addr + b * UNIT, pk);
+          tmem_st_wait();
+          tc_fence_before();
           __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->p_full[x][b]);
         }
       }
-    } else if (live) {  // no row of the tile sees a key
-      uint4* d4 = reinterpret_cast<uint4*>(dst);
+      units += n;
+      const int head = kvh * g + r - tok * g;
+      uint16_t* dst = out + static_cast<long long>(q_start + t) * p.ld_out + head * 128;
+      if (n > 0) {
+        ok = ok && mbar_wait_uniform(&bars->o_full[x], o_count & 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+        ++o_count;
+        if (ok) {
+          tc_fence_after();
+          const bool none = lsum == 0.f;
+          const float inv = none ? 0.f : 1.f / lsum;
+          float finite = 0.f;  // 0 times every output: NaN when one is not finite
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t rr[32];
+            tmem_ld32(o_addr + c * 32, rr);
+            float o[32];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) d4[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < 32; ++i) {
+              o[i] = __uint_as_float(rr[i]) * inv;
+              finite = fmaf(o[i], 0.f, finite);
+            }
+            if (live) {
+              uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                d4[i] = make_uint4(pack16<F16>(o[8 * i], o[8 * i + 1]), pack16<F16>(o[8 * i + 2], o[8 * i + 3]),
+                                   pack16<F16>(o[8 * i + 4], o[8 * i + 5]), pack16<F16>(o[8 * i + 6], o[8 * i + 7]));
+            }
+          }
+          tc_fence_before();  // O is read before the next item's first P lets an MMA write it
+          __syncwarp();
+          unsigned bad = __ballot_sync(0xffffffffu, live && finite != 0.f);
+          while (bad) {
+            const int src = __ffs(bad) - 1;
+            bad &= bad - 1;
+            const int rt = __shfl_sync(0xffffffffu, t, src), rh = __shfl_sync(0xffffffffu, head, src);
+            const int rl = __shfl_sync(0xffffffffu, lim, src);
+            const long long rows_end = p.kv_rows - k_start;  // rows past the tensor were read as zeros
+            const int last = static_cast<int>(min(static_cast<long long>(n) * UNIT, rows_end)) - 1;
+            const uint16_t* kb = static_cast<const uint16_t*>(p.k) + k_start * p.ld_k + kvh * 128;
+            const uint16_t* vb = static_cast<const uint16_t*>(p.v) + k_start * p.ld_v + kvh * 128;
+            mend_row<F16>(static_cast<const uint16_t*>(p.q) + static_cast<long long>(q_start + rt) * p.ld_q + rh * 128,
+                          kb, p.ld_k, vb, p.ld_v, rl, last, p.scale_log2,
+                          out + static_cast<long long>(q_start + rt) * p.ld_out + rh * 128);
+            __syncwarp();
+          }
+        }
+      } else if (live) {  // no row of the tile sees a key
+        uint4* d4 = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d4[i] = make_uint4(0u, 0u, 0u, 0u);
+      }
     }
   }
   tc_fence_before();
