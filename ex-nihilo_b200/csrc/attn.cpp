@@ -240,6 +240,7 @@ int exn_attn_packed(exn_attn* a, int type, int heads, int kv_heads, int nseq, co
   p.ld_k = ld_k;
   p.ld_v = ld_v;
   p.ld_out = ld_out;
+  p.sms = a->sms;
   return launched(a, fn, packed_launch(p, a->d_status, static_cast<cudaStream_t>(stream)));
 }
 

@@ -1235,6 +1235,7 @@ int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, 
   p.ld_k = p.ld_v = static_cast<long long>(c.kv_heads) * 128;
   p.ld_out = a.ld_out;
   p.scale_log2 = a.scale_log2;
+  p.sms = sms;
   return packed_launch(p, d_status, st);
 }
 

@@ -19,6 +19,9 @@
 // One CTA an SM takes items one after another, the longest first within a sequence: the grid has a CTA an
 // item, and a running CTA takes over those that have not started (cluster launch control), so the SMs
 // stay evenly loaded without a counter in memory, and barriers, TMEM and tensor maps are set up once.
+// SPLIT: where there are too few items of long sequences for the SMs, a cluster of 2, 4 or 8 CTAs shares
+// an item, each a part of its keys, and joins the parts through shared memory: with row maxima m_c,
+// sums l_c and outputs o_c of the parts and M = max m_c, o = sum 2^(m_c - M) o_c / sum 2^(m_c - M) l_c.
 // Roles, as in the single-sequence kernel of attention.cu:
 //   warp 0      finds the next item; TMA: Q_a, Q_b once an item; K_t, V_t through a ring of 4 slots, the next
 //               item's behind the last one's
@@ -68,6 +71,7 @@ struct Item {
   int q_start, nq, t0, tiles;  // the sequence's first query row and rows, the item's first token and tiles
   int delta, nu[2], nloads;    // token t sees keys 0 .. t + delta; units of each tile; 128-key loads
   int kvh;                     // key/value head; -1: no more items
+  int key0;                    // a cluster's CTA: its first key
   int k_start;                 // the sequence's first key row
 };
 
@@ -104,6 +108,19 @@ __device__ __forceinline__ int claim_answer(const void* src) {
       : "r"(smem_u32(src))
       : "memory");
   return got ? x : -1;
+}
+
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+__device__ __forceinline__ void st_cluster_f2(uint32_t addr, float a, float b) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
 }
 
 static_assert(sizeof(Bars) <= 512, "the barriers' room");
@@ -171,7 +188,7 @@ __device__ __noinline__ void mend_row(const uint16_t* q, const uint16_t* k, long
       make_uint2(pack16<F16>(o[0] * inv, o[1] * inv), pack16<F16>(o[2] * inv, o[3] * inv));
 }
 
-template <bool F16>
+template <bool F16, bool SPLIT>
 __global__ void __launch_bounds__(PK_THREADS, 1)
     k_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
              const __grid_constant__ CUtensorMap tmV, const PackedArgs p, int tpt, int nslots, int* status) {
@@ -185,6 +202,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = p.heads / p.kv_heads;
   uint16_t* const out = static_cast<uint16_t*>(p.out);
+  const int parts = SPLIT ? static_cast<int>(cluster_nctarank()) : 1, part = SPLIT ? static_cast<int>(cluster_ctarank()) : 0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(&bars->slot_full[i], 1);
@@ -233,6 +251,8 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     return mbar_wait(bar, parity, &none, status, STATUS_TIMEOUT_ATTN, 16 * EXN_WAIT_NS);
   };
 
+  float join_m = -INFINITY, join_l = 0.f;
+  bool has_o = false;
   if (warp == 0) {
     // ---- the items.  Sequence s owns the pair slots from floor(start_s / (2 tpt)) + s on; the distance to the
     // next sequence's first slot is at least ceil(length / (2 tpt)), so the host knows the count of slots
@@ -249,10 +269,6 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         hi = min(hi, lo + step);
       }
       const int a = p.q_offsets[lo], b = p.q_offsets[lo + 1];
-      x.t0 = (sl - (a / pair + lo)) * pair;
-      if (a < 0 || b > p.rows || x.t0 < 0 || x.t0 >= b - a) return false;
-      x.q_start = a;
-      x.nq = b - a;
       long long k_start;
       int nk;
       if (p.kv_lens) {
@@ -262,6 +278,10 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         k_start = p.kv_offsets[lo];
         nk = p.kv_offsets[lo + 1] - static_cast<int>(k_start);
       }
+      x.t0 = (sl - (a / pair + lo)) * pair;
+      if (a < 0 || b > p.rows || x.t0 < 0 || x.t0 >= b - a) return false;
+      x.q_start = a;
+      x.nq = b - a;
       if (k_start < 0 || nk < 0 || k_start + nk > p.kv_rows) {
         if (lane == 0) atomicOr(status, STATUS_BAD_ARG);
         return false;
@@ -276,12 +296,20 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         x.nu[i] = seen > 0 ? (seen + UNIT - 1) / UNIT : 0;
       }
       x.nloads = (max(x.nu[0], x.nu[1]) + 1) / 2;
+      x.key0 = 0;
+      if (SPLIT) {  // this CTA's share of the 128-key loads
+        const int l0 = x.nloads * part / parts, l1 = x.nloads * (part + 1) / parts;
+        x.key0 = l0 * TILE;
+        x.nloads = l1 - l0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x.nu[i] = min(max(x.nu[i] - 2 * l0, 0), 2 * (l1 - l0));
+      }
       return true;
     };
     // The next item is asked for late: near the end of the item at hand, and not in the kernel's first
     // microseconds, when the CTAs that have not started are still finding SMs of their own.
     uint32_t claims = 0;
-    bool ok = true, asked = false, ended = false;
+    bool ok = true, asked = false, ended = SPLIT;
     const uint64_t t_start = globaltimer();
     auto settled = [&] { return __any_sync(0xffffffffu, globaltimer() - t_start > 3000); };
     auto ask = [&] {
@@ -315,7 +343,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       tma_prefetch(&tmV);
     }
     Item cur;
-    if (!find(static_cast<int>(blockIdx.x), cur)) next_item(cur);
+    if (!find(static_cast<int>(blockIdx.x) / parts, cur)) next_item(cur);
     uint32_t q_count[2] = {0, 0}, loads = 0;  // so far
     for (uint32_t k = 0;; ++k) {
       const int ib = k & 1;
@@ -355,7 +383,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
           const CUtensorMap* map = (t & 1) ? &tmV : &tmK;
           for (int hf = 0; hf < 2; ++hf)
             tma_load_2d(smem + OFF_SLOT + sl * TILE_BYTES + hf * HALF, map, &bars->slot_full[sl], cur.kvh * 128 + hf * 64,
-                        cur.k_start + (t >> 1) * TILE);
+                        cur.k_start + cur.key0 + (t >> 1) * TILE);
         }
         ++loads;
       }
@@ -471,13 +499,13 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       const int ib = k & 1;
       if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->item_full[ib], (k >> 1) & 1) : true, 0)) break;
       const Item& it = bars->item[ib];
-      const int kvh = it.kvh, n = it.nu[x], n_a = it.nu[0], tiles = it.tiles, delta = it.delta, nq = it.nq;
+      const int kvh = it.kvh, n = it.nu[x], n_a = it.nu[0], tiles = it.tiles, delta = it.delta, nq = it.nq, it_key0 = it.key0;
       const int t = it.t0 + x * tpt + tok, q_start = it.q_start, k_start = it.k_start;  // t: token within the sequence
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->item_empty[ib]);
       if (kvh < 0) break;
       const bool live = tok < tpt && t < nq && x < tiles;
-      const int lim = live ? t + delta : n * UNIT;  // last visible key (< 0: none)
+      const int lim = live ? t + delta - it_key0 : n * UNIT;  // last visible key from KEY0 on (< 0: none)
       float m = -INFINITY, lsum = 0.f;
       const int turns = tiles == 2 ? n_a : 0;
       if (turns > 0 && x == 1) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");  // tile a goes first
@@ -562,6 +590,14 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         }
       }
       units += n;
+      if (SPLIT) {  // the join is behind the roles
+        if (n > 0) ok = ok && mbar_wait_uniform(&bars->o_full[x], 0, abort_flag, status, STATUS_TIMEOUT_ATTN);
+        tc_fence_after();
+        join_m = m;
+        join_l = lsum;
+        has_o = n > 0 && ok;
+        continue;
+      }
       const int head = kvh * g + r - tok * g;
       uint16_t* dst = out + static_cast<long long>(q_start + t) * p.ld_out + head * 128;
       if (n > 0) {
@@ -617,9 +653,73 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  tc_fence_after();
+  // ---- the join of a cluster's parts.  Every CTA owns PER rows: all send their share of O (fp32) and (m, l) there,
+  // over Q's and the ring's memory (16 bytes i of the owner's row j at i ^ (j % 32)), and the owner joins them, a
+  // warp a row.
+  const Item& it = bars->item[0];  // all the cluster's CTAs have the same item, or none
+  if (SPLIT) {
+    const int per = 2 * TILE / parts;
+    float2* const ml = reinterpret_cast<float2*>(smem + OFF_SLOT + 2 * TILE_BYTES);
+    cluster_sync();  // every CTA's MMAs are done
+    if (warp >= 3 && it.kvh >= 0) {
+      const int x = (warp - 3) >> 2, row = x * TILE + (warp & 3) * 32 + lane, j = row % per, owner = row / per;
+      const uint32_t o_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 + x * 128;
+      const uint32_t dst = mapa_shared(smem + (part * per + j) * 512, owner);
+      const int swz = j & 31;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        uint32_t rr[32];
+        if (__all_sync(0xffffffffu, has_o)) {
+          tmem_ld32(o_addr + c * 32, rr);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) rr[i] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) st_cluster_v4(dst + (((c * 8 + i) ^ swz) << 4), rr + 4 * i);
+      }
+      st_cluster_f2(mapa_shared(ml + part * per + j, owner), join_m, join_l);
+    }
+    cluster_sync();
+    if (warp >= 3 && it.kvh >= 0) {
+#pragma unroll 1
+      for (int j = warp - 3; j < per; j += 8) {
+        const int row = part * per + j, x = row / TILE, r = row - x * TILE, tok = r / g, t = it.t0 + x * tpt + tok;
+        if (x >= it.tiles || tok >= tpt || t >= it.nq) continue;
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < parts; ++c) m = fmaxf(m, ml[c * per + j].x);
+        const float mu = m == -INFINITY ? 0.f : m;
+        for (int c = 0; c < parts; ++c) {
+          const float2 y = ml[c * per + j];
+          const float4 z = reinterpret_cast<const float4*>(smem + (c * per + j) * 512)[lane ^ (j & 31)];
+          const float w = fast_exp2(y.x - mu);
+          l += w * y.y;
+          o.x += w * z.x;
+          o.y += w * z.y;
+          o.z += w * z.z;
+          o.w += w * z.w;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        const int head = it.kvh * g + r - tok * g;
+        uint16_t* const dst = out + static_cast<long long>(it.q_start + t) * p.ld_out + head * 128;
+        reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack16<F16>(o.x, o.y), pack16<F16>(o.z, o.w));
+        if (__any_sync(0xffffffffu, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)))) {
+          const int lim = t + it.delta, seen = min(it.nq, it.t0 + (x + 1) * tpt) + it.delta;  // by the tile's last row
+          const long long end = min((seen + static_cast<long long>(UNIT) - 1) / UNIT * UNIT, p.kv_rows - it.k_start);
+          const long long k0 = it.k_start;
+          mend_row<F16>(static_cast<const uint16_t*>(p.q) + static_cast<long long>(it.q_start + t) * p.ld_q + head * 128,
+                        static_cast<const uint16_t*>(p.k) + k0 * p.ld_k + it.kvh * 128, p.ld_k,
+                        static_cast<const uint16_t*>(p.v) + k0 * p.ld_v + it.kvh * 128, p.ld_v, lim,
+                        static_cast<int>(end) - 1, p.scale_log2, dst);
+        }
+      }
+    }
+  }
   if (warp == 1) {
     __syncwarp();
-    tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
 }
@@ -627,9 +727,9 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
 }  // namespace
 
 int packed_prepare() {
-  cudaError_t e = cudaFuncSetAttribute(k_packed<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PK_SMEM);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_packed<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PK_SMEM);
-  return static_cast<int>(e);
+  for (auto* kernel : {k_packed<false, false>, k_packed<true, false>, k_packed<false, true>, k_packed<true, true>})
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PK_SMEM) != cudaSuccess) return -4;
+  return 0;
 }
 
 int packed_launch(const PackedArgs& a, int* d_status, cudaStream_t st) {
@@ -648,11 +748,39 @@ int packed_launch(const PackedArgs& a, int* d_status, cudaStream_t st) {
       make_tmap(&tk, type, a.k, 2, dk, sk, bk, CU_TENSOR_MAP_SWIZZLE_128B) ||
       make_tmap(&tv, type, a.v, 2, dk, sv, bk, CU_TENSOR_MAP_SWIZZLE_128B))
     return -4;
-  const long long nslots = a.rows / (2 * tpt) + a.nseq;
-  if (nslots * a.kv_heads > 0x7fffffffll) return -1;
-  return static_cast<int>(launch_pdl(a.f16 ? k_packed<true> : k_packed<false>,
-                                     dim3(static_cast<unsigned>(nslots * a.kv_heads)), dim3(PK_THREADS), PK_SMEM, st, tq,
-                                     tk, tv, a, tpt, static_cast<int>(nslots), d_status));
+  const long long nslots = a.rows / (2 * tpt) + a.nseq, items = nslots * a.kv_heads;  // items, at most
+  if (items > 0x7fffffffll) return -1;
+  // CTAs an item.  A cluster's launch and join cost about 10 us, so it has to have keys enough to share, and its
+  // CTAs fit the SMs at once; clusters of 8 leave a few SMs of each group unused.  us at 1, 2, 4 and 8 CTAs an
+  // item (32 heads over 8, bf16):
+  //   64 rows (8 items)    over  1024 keys:  22   25   20   21    over 16384 keys: 249  138   76   49
+  //   192 rows (32 items)  over  1024 keys:  23   26   21   38    over  8192 keys: 128   78   48   65
+  //   512 rows (72 items)  over  1024 keys:  23   26   42   87    over  8192 keys: 130   80   96  153
+  const long long keys = a.kv_rows / a.nseq;
+  int parts = 1;
+  if (keys >= 1024 && items * 8 <= a.sms * 7ll / 8)
+    parts = 8;
+  else if (keys >= 1024 && items * 4 <= a.sms)
+    parts = 4;
+  else if (keys >= 2048 && items * 2 <= a.sms)
+    parts = 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * parts));
+  cfg.blockDim = dim3(PK_THREADS);
+  cfg.dynamicSmemBytes = PK_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = parts;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = parts > 1 ? 2 : 1;
+  auto* const kernel = parts > 1 ? (a.f16 ? k_packed<true, true> : k_packed<false, true>)
+                                 : (a.f16 ? k_packed<true, false> : k_packed<false, false>);
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, tq, tk, tv, a, tpt, static_cast<int>(nslots), d_status));
 }
 
 }  // namespace exn

@@ -395,6 +395,7 @@ int attend_sequences(exn_enc* e, int li, int n, const Scratch& s, const Pass& ps
     a.ld_q = a.ld_out = q;
     a.ld_k = a.ld_v = kv;
     a.scale_log2 = scale_log2;
+    a.sms = e->sms;
     r = packed_launch(a, e->d_status, e->st);
   } else {
     CacheAttnArgs a;

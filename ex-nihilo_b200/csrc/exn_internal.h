@@ -153,6 +153,7 @@ struct PackedArgs {
   void* out = nullptr;
   long long ld_q = 0, ld_k = 0, ld_v = 0, ld_out = 0;
   float scale_log2 = 0.f;
+  int sms = 148;
 };
 int packed_launch(const PackedArgs& a, int* d_status, cudaStream_t st);
 int packed_prepare();

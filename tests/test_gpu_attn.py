@@ -210,6 +210,44 @@ def test_packed_deterministic_and_independent_of_the_packing(att):
     assert torch.equal(a[37:187], b)
 
 
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (28, 4), (5, 1), (16, 16)])
+@pytest.mark.parametrize("nq,nk", [([64], [5000]), ([1], [1024]), ([70, 3, 40], [4200, 0, 1500]), ([129, 0], [2049, 63]),
+                                   ([300, 77], [4100, 900])])
+def test_packed_few_rows_over_long_keys(att, heads, kv_heads, t, nq, nk):
+    """Few work items of long sequences, whose keys several blocks share: from a share of one load to many,
+    a last share that only the item's later rows see, a sequence without keys beside long ones."""
+    q, k, v = rows(sum(nq), heads, 1, t), rows(sum(nk), kv_heads, 2, t), rows(sum(nk), kv_heads, 3, t)
+    out = run_packed(att, q, k, v, nq, heads, kv_heads, t, nk=nk)
+    check_packed(out, q, k, v, nq, heads, kv_heads, t, nk=nk)
+    assert torch.equal(out, run_packed(att, q, k, v, nq, heads, kv_heads, t, nk=nk))
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_packed_shared_keys_that_are_not_finite(att, t, value):
+    """As above for a value row that is not finite among the last tokens of a long sequence, and for a key
+    row in the middle: rows that do not see the value row keep their bits, those that do are not finite in
+    its dim; a key row that is NaN reaches every row of its heads."""
+    nq, nk, heads, kv_heads = [70, 40], [2050, 1500], 8, 2
+    q, k, v = rows(110, heads, 1, t), rows(3550, kv_heads, 2, t), rows(3550, kv_heads, 3, t)
+    good = run_packed(att, q, k, v, nq, heads, kv_heads, t, nk=nk)
+    bad = v.clone()
+    bad[2050 - 20, 5] = value  # row 50's own token
+    out = run_packed(att, q, k, bad, nq, heads, kv_heads, t, nk=nk)
+    check(out[:50], tuple(x[:50] for x in reference(q[:70], k[:2050], v[:2050], heads, kv_heads)), t)
+    dims = torch.zeros(heads * D, dtype=torch.bool, device="cuda")
+    dims[torch.arange(4, device="cuda") * D + 5] = True
+    assert not torch.isfinite(out[50:70][:, dims]).any()
+    assert torch.equal(out[50:70][:, ~dims], good[50:70][:, ~dims]) and torch.equal(out[70:], good[70:])
+    bad = k.clone()
+    bad[700, 5] = value
+    out = run_packed(att, q, bad, v, nq, heads, kv_heads, t, nk=nk)
+    assert torch.equal(out[:, 4 * D:], good[:, 4 * D:]) and torch.equal(out[70:], good[70:])
+    if value != value:
+        assert torch.isnan(out[:70, :4 * D]).all()
+
+
 # --------------------------------------------------------------------------- the cache
 
 
