@@ -54,89 +54,89 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cas
 
 __device__ __forceinline__ int to_code(float x, float top) { return __float2int_rn(fminf(fmaxf(x, -top), top)); }
 
-// The sequence whose page slots hold SLOT: s owns the slots from floor(start_s / 64) + 2 s on, of which
-// its rows, consecutive positions, touch at most ceil(count / 64) + 1 pages.  All threads; -1: none.
-__device__ __forceinline__ int find_sequence(const int* offsets, const int* lens, int nseq, long long rows, int slot,
-                                             int* found, int* status) {
-  if (threadIdx.x == 0) *found = -1;
+// The rows of a call that fall into one page, by the page's slot: sequence s owns the slots from
+// floor(start_s / 64) + 2 s on, of which its rows, consecutive positions, touch at most ceil(count / 64) + 1.
+struct PageRows {
+  int s, page_i;    // the sequence (-1: none) and its page
+  int lo, hi;       // the page's rows of this call: lo .. hi - 1
+  long long row0;   // the row of the page's position 0 (below 0 where the call starts inside the page)
+};
+// all threads; FOUND is shared by the block
+__device__ __forceinline__ void find_page(const int* offsets, const int* lens, int nseq, long long rows, int slot,
+                                          PageRows* found, int* status) {
+  if (threadIdx.x == 0) found->s = -1;
   __syncthreads();
   for (int s = threadIdx.x; s < nseq; s += blockDim.x) {
-    const long long a = offsets[s], b = offsets[s + 1];
-    if (a < 0 || b < a || b > rows || lens[s] < b - a) {
+    const int a = offsets[s], b = offsets[s + 1], len = lens[s];
+    if (a < 0 || b < a || b > rows || len < b - a) {
       if (blockIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
       continue;
     }
     if (b == a) continue;
-    const long long first = a / kPage + 2ll * s;
-    const long long p0 = (lens[s] - (b - a)) / kPage, p1 = (lens[s] - 1) / kPage;
-    if (slot >= first && slot <= first + p1 - p0) *found = s;
+    const int pos0 = len - (b - a), p0 = pos0 / kPage, p1 = (len - 1) / kPage;
+    const long long i = slot - (a / kPage + 2ll * s);
+    if (i < 0 || i > p1 - p0) continue;
+    const int page_i = p0 + static_cast<int>(i);
+    const long long base = static_cast<long long>(page_i) * kPage;
+    found->s = s;
+    found->page_i = page_i;
+    found->lo = static_cast<int>(max(pos0 - base, 0ll));
+    found->hi = static_cast<int>(min(len - base, static_cast<long long>(kPage)));
+    found->row0 = a + base - pos0;
   }
   __syncthreads();
-  return *found;
 }
 
 // ---- write: one block = one page touched by the call's rows, one key/value head; threads 0..127 take
-// K, 128..255 V, eight threads a row of 128 values.  Bound by the bytes: 2 in and 1 out a value.
+// K, 128..255 V, 16 threads a row of 128 values.  Long prompts are bound by the bytes, 2 in and 1 out a
+// value; single tokens by the chain of dependent loads (offsets and lengths; the rows and the table's
+// entry; the page's scale; its codes, when the scale grows).
 template <bool F16>
 __global__ void __launch_bounds__(256) k_cache_write(const CacheArgs c, const int* __restrict__ offsets,
                                                      long long rows, const uint16_t* __restrict__ k, long long ld_k,
                                                      const uint16_t* __restrict__ v, long long ld_v, int* status) {
-  __shared__ int found;
-  __shared__ float red[8];
+  __shared__ PageRows at;
+  __shared__ uint32_t red[8];
   const int slot = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads;
   griddep_wait();
   griddep_launch();
-  const int s = find_sequence(offsets, c.lens, c.nseq, rows, slot, &found, status);
-  if (s < 0) return;
-  const int start = offsets[s], count = offsets[s + 1] - start;
-  const int pos0 = c.lens[s] - count;
-  const int page_i = pos0 / kPage + slot - (start / kPage + 2 * s);
-  const int page = page_i < c.table_ld ? c.table[static_cast<long long>(s) * c.table_ld + page_i] : -1;
+  find_page(offsets, c.lens, c.nseq, rows, slot, &at, status);
+  if (at.s < 0) return;
+  const int page = at.page_i < c.table_ld ? c.table[static_cast<long long>(at.s) * c.table_ld + at.page_i] : -1;
+  const int lo = at.lo, hi = at.hi;
+  const bool is_v = threadIdx.x >= 128;
+  const int tid = threadIdx.x & 127, sub = tid & 15, r0 = tid >> 4;  // 8 values at 8 sub of rows r0, r0 + 8, ..
+  const long long ld = is_v ? ld_v : ld_k;
+  const uint16_t* src = (is_v ? v : k) + at.row0 * ld + h * 128 + sub * 8;
+
+  uint4 x[8];
+  uint32_t mag = 0;  // the largest magnitudes of the even and odd values, as bits: their order is that of the values
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 8 * i;
+    x[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (r >= lo && r < hi) x[i] = __ldg(reinterpret_cast<const uint4*>(src + r * ld));
+  }
   if (page < 0 || page >= c.pages) {
     if (threadIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
     return;
   }
-  const int lo = max(pos0, page_i * kPage) - page_i * kPage;             // rows of the page written: lo .. hi - 1
-  const int hi = min(pos0 + count, (page_i + 1) * kPage) - page_i * kPage;
-  const long long row0 = start + static_cast<long long>(page_i) * kPage - pos0;  // the row of the page's position 0
-  const bool is_v = threadIdx.x >= 128;
-  const int tid = threadIdx.x & 127, sub = tid & 7, r0 = tid >> 3;  // 16 values at 16 sub of rows r0, r0 + 16, ..
-  const uint16_t* src = (is_v ? v : k) + h * 128 + sub * 16;
-  const long long ld = is_v ? ld_v : ld_k;
   const long long head = static_cast<long long>(page) * c.kv_heads + h;
-  int8_t* dst = (is_v ? c.v : c.k) + head * PAGE_BYTES + sub * 16;
+  int8_t* dst = (is_v ? c.v : c.k) + head * PAGE_BYTES + sub * 8;
   float* scale = (is_v ? c.v_scale : c.k_scale) + head;
-
-  uint4 x[4][2];
-  float amax = 0.f;
-  bool bad = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + 16 * i;
-    x[i][0] = x[i][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (r >= lo && r < hi) {
-      const uint4* p = reinterpret_cast<const uint4*>(src + (row0 + r) * ld);
-      x[i][0] = __ldg(p);
-      x[i][1] = __ldg(p + 1);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float2 f = unpack16<F16>(reinterpret_cast<const uint32_t*>(&x[i][0])[j]);
-      amax = fmax3(amax, fabsf(f.x), fabsf(f.y));
-      bad |= !(fabsf(f.x) < INFINITY) || !(fabsf(f.y) < INFINITY);
-    }
-  if (bad) amax = INFINITY;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
   const float before = lo > 0 ? *scale : 0.f;  // what the page holds already (none when it starts anew)
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mag = __vmaxu2(mag, reinterpret_cast<const uint32_t*>(&x[i])[j] & 0x7fff7fffu);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mag = __vmaxu2(mag, __shfl_xor_sync(0xffffffffu, mag, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mag;
   __syncthreads();
   const int w0 = is_v ? 4 : 0;
-  amax = fmaxf(fmaxf(red[w0], red[w0 + 1]), fmaxf(red[w0 + 2], red[w0 + 3]));
-  const bool poisoned = !(amax < INFINITY) || before != before;
+  mag = __vmaxu2(__vmaxu2(red[w0], red[w0 + 1]), __vmaxu2(red[w0 + 2], red[w0 + 3]));
+  const float amax = unpack16<F16>(max(mag & 0xffffu, mag >> 16)).x;
+  const bool poisoned = !(amax < INFINITY) || before != before;  // infinite or NaN
   const float mine = pow2(scale_exponent(poisoned ? 0.f : amax));
   const float now = fmaxf(mine, before);
   const float inv = 1.f / now;  // exact: a power of two between 2^-122 and 2^126
@@ -144,14 +144,14 @@ __global__ void __launch_bounds__(256) k_cache_write(const CacheArgs c, const in
   if (lo > 0 && !poisoned && now > before) {  // the codes that are there, in the larger unit
     const float f = before * inv;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r0 + 16 * i;
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + 8 * i;
       if (r < lo) {
-        uint4* p = reinterpret_cast<uint4*>(dst + r * 128);
-        uint4 w = *p;
+        uint2* p = reinterpret_cast<uint2*>(dst + r * 128);
+        uint2 w = *p;
         uint32_t* u = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
           uint32_t n = 0;
 #pragma unroll
           for (int b = 0; b < 4; ++b) {
@@ -165,23 +165,25 @@ __global__ void __launch_bounds__(256) k_cache_write(const CacheArgs c, const in
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + 16 * i;
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 8 * i;
     if (r >= lo && r < hi) {
-      uint4 w;
-      uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+      uint32_t u[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 a = unpack16<F16>(reinterpret_cast<const uint32_t*>(&x[i][0])[2 * j]);
-        const float2 b = unpack16<F16>(reinterpret_cast<const uint32_t*>(&x[i][0])[2 * j + 1]);
-        const float f[4] = {a.x, a.y, b.x, b.y};
-        uint32_t n = 0;
+      for (int j = 0; j < 2; ++j) {
+        const float2 a = unpack16<F16>(reinterpret_cast<const uint32_t*>(&x[i])[2 * j]);
+        const float2 b = unpack16<F16>(reinterpret_cast<const uint32_t*>(&x[i])[2 * j + 1]);
+        float f[4] = {a.x, a.y, b.x, b.y};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          n |= (static_cast<uint32_t>(poisoned ? 0 : to_code(f[e] * inv, top)) & 0xffu) << (8 * e);
+        for (int e = 0; e < 4; ++e) {
+          f[e] = fmaf(f[e], inv, 0x1.8p23f);  // rounded to an integer, which is then the low bits
+          if (top != 127.f) f[e] = fminf(fmaxf(f[e], 0x1.8p23f - top), 0x1.8p23f + top);
+        }
+        const uint32_t n = poisoned ? 0u : __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
+                                                       __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
         u[j] = n;
       }
-      *reinterpret_cast<uint4*>(dst + r * 128) = w;
+      *reinterpret_cast<uint2*>(dst + r * 128) = make_uint2(u[0], u[1]);
     }
   }
   if (tid == 0) *scale = poisoned ? __uint_as_float(0x7fffffffu) : now;
@@ -193,67 +195,59 @@ template <bool F16, bool DENSE>
 __global__ void __launch_bounds__(256) k_cache_read(const CacheArgs c, const int* __restrict__ offsets,
                                                     long long rows, uint16_t* __restrict__ k, long long ld_k,
                                                     uint16_t* __restrict__ v, long long ld_v, int* status) {
-  __shared__ int found;
+  __shared__ PageRows found;
   const int slot = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads;
   griddep_wait();
   griddep_launch();
-  int s, page_i, lo, hi;
-  long long row0;
+  PageRows at;
   if (DENSE) {
-    s = slot / c.table_ld;
-    page_i = slot - s * c.table_ld;
-    const int len = c.lens[s];
+    at.s = slot / c.table_ld;
+    at.page_i = slot - at.s * c.table_ld;
+    const int len = c.lens[at.s];
     if (len < 0 || len > static_cast<long long>(c.table_ld) * kPage) {
-      if (page_i == 0 && threadIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
+      if (at.page_i == 0 && threadIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
       return;
     }
-    if (len <= page_i * kPage) return;
-    lo = 0;  // the last page whole: the rows behind the sequence's last are then finite, as its codes are
-    hi = kPage;
-    row0 = static_cast<long long>(slot) * kPage;
+    if (len <= at.page_i * kPage) return;
+    at.lo = 0;  // the last page whole: the rows behind the sequence's last are then finite, as its codes are
+    at.hi = kPage;
+    at.row0 = static_cast<long long>(slot) * kPage;
   } else {
-    s = find_sequence(offsets, c.lens, c.nseq, rows, slot, &found, status);
-    if (s < 0) return;
-    const int start = offsets[s], count = offsets[s + 1] - start;
-    const int pos0 = c.lens[s] - count;
-    page_i = pos0 / kPage + slot - (start / kPage + 2 * s);
-    lo = max(pos0, page_i * kPage) - page_i * kPage;
-    hi = min(pos0 + count, (page_i + 1) * kPage) - page_i * kPage;
-    row0 = start + static_cast<long long>(page_i) * kPage - pos0;
+    find_page(offsets, c.lens, c.nseq, rows, slot, &found, status);
+    at = found;
+    if (at.s < 0) return;
   }
-  const int page = page_i < c.table_ld ? c.table[static_cast<long long>(s) * c.table_ld + page_i] : -1;
+  const int page = at.page_i < c.table_ld ? c.table[static_cast<long long>(at.s) * c.table_ld + at.page_i] : -1;
   if (page < 0 || page >= c.pages) {
     if (threadIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
     return;
   }
   const bool is_v = threadIdx.x >= 128;
-  const int tid = threadIdx.x & 127, sub = tid & 7, r0 = tid >> 3;
+  const int tid = threadIdx.x & 127, sub = tid & 15, r0 = tid >> 4;
   const long long head = static_cast<long long>(page) * c.kv_heads + h;
-  const int8_t* src = (is_v ? c.v : c.k) + head * PAGE_BYTES + sub * 16;
+  const int8_t* src = (is_v ? c.v : c.k) + head * PAGE_BYTES + sub * 8;
   const float scale = (is_v ? c.v_scale : c.k_scale)[head];
-  uint16_t* dst = (is_v ? v : k) + h * 128 + sub * 16;
   const long long ld = is_v ? ld_v : ld_k;
-  uint4 w[4];
+  uint16_t* dst = (is_v ? v : k) + at.row0 * ld + h * 128 + sub * 8;
+  uint2 w[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + 16 * i;
-    if (r >= lo && r < hi) w[i] = *reinterpret_cast<const uint4*>(src + r * 128);
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 8 * i;
+    if (r >= at.lo && r < at.hi) w[i] = *reinterpret_cast<const uint2*>(src + r * 128);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + 16 * i;
-    if (r < lo || r >= hi) continue;
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 8 * i;
+    if (r < at.lo || r >= at.hi) continue;
     const uint32_t* u = reinterpret_cast<const uint32_t*>(&w[i]);
-    uint32_t o[8];
+    uint32_t o[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 4; ++j) {
       const uint32_t pair = u[j >> 1] >> (16 * (j & 1));
       o[j] = pack16<F16>(static_cast<float>(static_cast<int8_t>(pair)) * scale,
                          static_cast<float>(static_cast<int8_t>(pair >> 8)) * scale);
     }
-    uint4* p = reinterpret_cast<uint4*>(dst + (row0 + r) * ld);
-    p[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    *reinterpret_cast<uint4*>(dst + r * ld) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
