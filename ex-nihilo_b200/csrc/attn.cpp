@@ -5,8 +5,8 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstring>
 #include <new>
-#include <string>
 
 #include "../../include/exn_b200.h"
 #include "exn_internal.h"
@@ -14,22 +14,20 @@
 using namespace exn;
 
 struct exn_attn {
-  int device = 0, sms = 0;
+  int device = 0, sms = 0, fit[3] = {0, 0, 0};
   int* d_status = nullptr;
-  std::string err;
+  char err[512] = "";  // no allocation, so no exception either, on the way to the caller
 };
 
 namespace {
 
-thread_local std::string g_attn_open_error;
+thread_local char g_attn_open_error[512];
 
 int afail(exn_attn* a, int code, const char* fmt, ...) {
-  char buf[512];
   va_list ap;
   va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
+  vsnprintf(a ? a->err : g_attn_open_error, 512, fmt, ap);
   va_end(ap);
-  (a ? a->err : g_attn_open_error) = buf;
   return code;
 }
 
@@ -155,12 +153,12 @@ int exn_attn_open(int device, exn_attn** out) {
     ACK(on.rc);
     ACK(cudaMalloc(&a->d_status, sizeof(int)));
     ACK(cudaMemset(a->d_status, 0, sizeof(int)));
-    ACK(static_cast<cudaError_t>(packed_prepare()));
+    ACK(static_cast<cudaError_t>(packed_prepare(a->fit)));
     ACK(static_cast<cudaError_t>(cache_prepare()));
     return EXN_OK;
   }();
   if (rc) {
-    g_attn_open_error = a->err;
+    memcpy(g_attn_open_error, a->err, sizeof a->err);
     exn_attn_close(a);
     return rc;
   }
@@ -177,7 +175,7 @@ void exn_attn_close(exn_attn* a) {
   delete a;
 }
 
-const char* exn_attn_last_error(const exn_attn* a) { return a ? a->err.c_str() : g_attn_open_error.c_str(); }
+const char* exn_attn_last_error(const exn_attn* a) { return a ? a->err : g_attn_open_error; }
 
 int exn_attn_sync(exn_attn* a, void* stream) {
   if (!a) return afail(a, EXN_EINVAL, "exn_attn_sync: null handle");
@@ -240,7 +238,7 @@ int exn_attn_packed(exn_attn* a, int type, int heads, int kv_heads, int nseq, co
   p.ld_k = ld_k;
   p.ld_v = ld_v;
   p.ld_out = ld_out;
-  p.sms = a->sms;
+  for (int i = 0; i < 3; ++i) p.fit[i] = a->fit[i];
   return launched(a, fn, packed_launch(p, a->d_status, static_cast<cudaStream_t>(stream)));
 }
 
@@ -320,7 +318,7 @@ int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int 
   p.ld_q = ld_q;
   p.out = out;
   p.ld_out = ld_out;
-  return launched(a, fn, cache_attention(p, workspace, workspace_bytes, a->sms, a->d_status, st));
+  return launched(a, fn, cache_attention(p, workspace, workspace_bytes, a->sms, a->fit, a->d_status, st));
 }
 
 }  // extern "C"

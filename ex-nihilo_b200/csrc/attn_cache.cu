@@ -14,7 +14,7 @@
 // that is given an infinity or a NaN gets the scale NaN and makes NaN of what
 // is read from it until it starts anew at its first position.
 #include <atomic>
-#include <random>
+#include <chrono>
 
 #include "exn_device.cuh"
 #include "exn_internal.h"
@@ -1103,7 +1103,8 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
 
 // A number that no other launch of this process has and that is no likely memory content
 unsigned long long launch_tag() {
-  static std::atomic<unsigned long long> next{std::random_device{}() * 0x9e3779b97f4a7c15ull};
+  static std::atomic<unsigned long long> next{
+      static_cast<unsigned long long>(std::chrono::system_clock::now().time_since_epoch().count()) * 0x9e3779b97f4a7c15ull};
   unsigned long long t;
   do t = next.fetch_add(0x9e3779b97f4a7c15ull) << 16;  // an odd step: every 48-bit number once
   while (t == 0);                                      // 0: no launch's
@@ -1148,13 +1149,16 @@ int cache_prepare() {
   return static_cast<int>(e);
 }
 
-// Rows (tokens times the query heads of a key/value head) a sequence, on average, beyond which the cache
-// is turned into 16 bits once and read by the packed kernel's tensor-core tiles; up to it, the codes are
-// read directly, 16 rows at a time.
-constexpr long long kDenseRows = 64;
-
+// Few rows (tokens times the query heads of a key/value head) read the codes directly, 16 at a time; with
+// more, the cache is turned into 16 bits once and read by the packed kernel's tensor-core tiles.  us either
+// way, codes / 16 bits (32 heads over 8):
+//   rows a sequence              32          64          96         128         192
+//   1 sequence of 8000       23 / 37     31 / 37     32 / 37     42 / 37     54 / 40
+//   8 sequences of 2000      24 / 44     47 / 50     62 / 50     76 / 51    105 / 53
+//   32 sequences of 4000    130 / 245   236 / 246   339 / 248   443 / 252   657 / 269
+// so the bound is 64 rows a sequence and 64 more for the launch.
 static bool dense_path(const CacheArgs& c, int heads, long long rows) {
-  return rows * (heads / c.kv_heads) > kDenseRows * c.nseq;
+  return rows * (heads / c.kv_heads) > 64 * (c.nseq + 1ll);
 }
 static long long dense_rows(const CacheArgs& c) { return static_cast<long long>(c.nseq) * c.table_ld * kPage; }
 
@@ -1202,7 +1206,8 @@ static int attend_launch(const CacheAttnArgs& a, void* ws, int sms, int* d_statu
                                      dim3(p.ctas), dim3(threads), smem, st, tk, tv, a, p, d_status));
 }
 
-int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, int* d_status, cudaStream_t st) {
+int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, const int (&fit)[3], int* d_status,
+                    cudaStream_t st) {
   const CacheArgs& c = a.c;
   if (ws_bytes < cache_attention_workspace(c, a.heads, a.rows, sms)) return -1;
   if (!dense_path(c, a.heads, a.rows)) return attend_launch(a, ws, sms, d_status, st);
@@ -1229,7 +1234,7 @@ int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, 
   p.ld_k = p.ld_v = static_cast<long long>(c.kv_heads) * 128;
   p.ld_out = a.ld_out;
   p.scale_log2 = a.scale_log2;
-  p.sms = sms;
+  for (int i = 0; i < 3; ++i) p.fit[i] = fit[i];
   return packed_launch(p, d_status, st);
 }
 

@@ -726,9 +726,37 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
 
 }  // namespace
 
-int packed_prepare() {
-  for (auto* kernel : {k_packed<false, false>, k_packed<true, false>, k_packed<false, true>, k_packed<true, true>})
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PK_SMEM) != cudaSuccess) return -4;
+// a launch of ITEMS clusters of PARTS CTAs that may start while the kernel before it ends
+struct PackedLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  PackedLaunch(unsigned items, int parts, cudaStream_t st) {
+    cfg.gridDim = dim3(items * parts);
+    cfg.blockDim = dim3(PK_THREADS);
+    cfg.dynamicSmemBytes = PK_SMEM;
+    cfg.stream = st;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = parts;
+    at[1].val.clusterDim.y = 1;
+    at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = parts > 1 ? 2 : 1;
+  }
+  PackedLaunch(const PackedLaunch&) = delete;
+};
+
+int packed_prepare(int (&fit)[3]) {
+  for (auto* kernel : {k_packed<false, false>, k_packed<true, false>, k_packed<false, true>, k_packed<true, true>}) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PK_SMEM);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
+  for (int i = 0; i < 3; ++i) {
+    PackedLaunch l(1, 2 << i, nullptr);
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&fit[i], k_packed<false, true>, &l.cfg);
+    if (e != cudaSuccess) return static_cast<int>(e);
+  }
   return 0;
 }
 
@@ -748,39 +776,20 @@ int packed_launch(const PackedArgs& a, int* d_status, cudaStream_t st) {
       make_tmap(&tk, type, a.k, 2, dk, sk, bk, CU_TENSOR_MAP_SWIZZLE_128B) ||
       make_tmap(&tv, type, a.v, 2, dk, sv, bk, CU_TENSOR_MAP_SWIZZLE_128B))
     return -4;
-  const long long nslots = a.rows / (2 * tpt) + a.nseq, items = nslots * a.kv_heads;  // items, at most
+  const long long nslots = (a.rows - 1) / (2 * tpt) + a.nseq, items = nslots * a.kv_heads;  // at most
   if (items > 0x7fffffffll) return -1;
-  // CTAs an item.  A cluster's launch and join cost about 10 us, so it has to have keys enough to share, and its
-  // CTAs fit the SMs at once; clusters of 8 leave a few SMs of each group unused.  us at 1, 2, 4 and 8 CTAs an
-  // item (32 heads over 8, bf16):
+  // CTAs an item.  A cluster's launch and join cost about 10 us, so it has to have keys enough to share, and all
+  // clusters run at once (74 of 2, 33 of 4, 15 of 8).  us at 1, 2, 4 and 8 CTAs an item (32 heads over 8, bf16):
   //   64 rows (8 items)    over  1024 keys:  22   25   20   21    over 16384 keys: 249  138   76   49
   //   192 rows (32 items)  over  1024 keys:  23   26   21   38    over  8192 keys: 128   78   48   65
   //   512 rows (72 items)  over  1024 keys:  23   26   42   87    over  8192 keys: 130   80   96  153
   const long long keys = a.kv_rows / a.nseq;
-  int parts = 1;
-  if (keys >= 1024 && items * 8 <= a.sms * 7ll / 8)
-    parts = 8;
-  else if (keys >= 1024 && items * 4 <= a.sms)
-    parts = 4;
-  else if (keys >= 2048 && items * 2 <= a.sms)
-    parts = 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * parts));
-  cfg.blockDim = dim3(PK_THREADS);
-  cfg.dynamicSmemBytes = PK_SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = parts;
-  at[1].val.clusterDim.y = 1;
-  at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = parts > 1 ? 2 : 1;
+  const int parts = keys >= 1024 && items <= a.fit[2] ? 8 : keys >= 1024 && items <= a.fit[1] ? 4
+                    : keys >= 2048 && items <= a.fit[0] ? 2 : 1;
+  const PackedLaunch l(static_cast<unsigned>(items), parts, st);
   auto* const kernel = parts > 1 ? (a.f16 ? k_packed<true, true> : k_packed<false, true>)
                                  : (a.f16 ? k_packed<true, false> : k_packed<false, false>);
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, tq, tk, tv, a, tpt, static_cast<int>(nslots), d_status));
+  return static_cast<int>(cudaLaunchKernelEx(&l.cfg, kernel, tq, tk, tv, a, tpt, static_cast<int>(nslots), d_status));
 }
 
 }  // namespace exn

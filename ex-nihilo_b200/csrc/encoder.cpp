@@ -75,7 +75,7 @@ struct EncLayer {
 
 struct exn_enc {
   exn_enc_config cfg{};
-  int sms = 0;
+  int sms = 0, fit[3] = {0, 0, 0};  // packed_prepare's
   cudaStream_t st = nullptr;
   int* d_status = nullptr;
   std::string err;
@@ -395,7 +395,7 @@ int attend_sequences(exn_enc* e, int li, int n, const Scratch& s, const Pass& ps
     a.ld_q = a.ld_out = q;
     a.ld_k = a.ld_v = kv;
     a.scale_log2 = scale_log2;
-    a.sms = e->sms;
+    for (int i = 0; i < 3; ++i) a.fit[i] = e->fit[i];
     r = packed_launch(a, e->d_status, e->st);
   } else {
     CacheAttnArgs a;
@@ -408,7 +408,7 @@ int attend_sequences(exn_enc* e, int li, int n, const Scratch& s, const Pass& ps
     a.out = s.xn;
     a.scale_log2 = scale_log2;
     r = cache_write_launch(a.c, 0, ps.offsets, n, s.k, kv, s.v, kv, e->d_status, e->st);
-    if (!r) r = cache_attention(a, ps.ws, ps.ws_bytes, e->sms, e->d_status, e->st);
+    if (!r) r = cache_attention(a, ps.ws, ps.ws_bytes, e->sms, e->fit, e->d_status, e->st);
   }
   if (r) return efail(e, EXN_ECUDA, "encoder block %d: attention (%d rows, %d sequences) launch failed: %d", li, n, ps.nseq, r);
   return EXN_OK;
@@ -585,7 +585,7 @@ int exn_enc_open(const exn_enc_config* cfg, exn_enc** out) {
     ECK(static_cast<cudaError_t>(gemm_prepare()));
     ECK(static_cast<cudaError_t>(attention_prepare()));
     ECK(static_cast<cudaError_t>(gemm_thin_prepare()));
-    ECK(static_cast<cudaError_t>(packed_prepare()));
+    ECK(static_cast<cudaError_t>(packed_prepare(e->fit)));
     ECK(static_cast<cudaError_t>(cache_prepare()));
     ECK(cudaEventCreate(&e->ev[0]));
     ECK(cudaEventCreate(&e->ev[1]));

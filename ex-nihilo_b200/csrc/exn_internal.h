@@ -153,10 +153,11 @@ struct PackedArgs {
   void* out = nullptr;
   long long ld_q = 0, ld_k = 0, ld_v = 0, ld_out = 0;
   float scale_log2 = 0.f;
-  int sms = 148;
+  int fit[3] = {0, 0, 0};  // packed_prepare's
 };
 int packed_launch(const PackedArgs& a, int* d_status, cudaStream_t st);
-int packed_prepare();
+// the kernels set up on the current device; FIT: how many clusters of 2, 4 and 8 CTAs run there at once
+int packed_prepare(int (&fit)[3]);
 
 // The 8-bit key/value cache (attn_cache.cu): exn_kv_cache of include/exn_b200.h
 constexpr int kPage = 64;  // tokens a page
@@ -184,7 +185,8 @@ struct CacheAttnArgs {
   float scale_log2 = 0.f;
 };
 // WS: cache_attention_workspace's bytes, 16-byte aligned.  0, -1 (size), -4 (tensor map) or a cudaError_t.
-int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, int* d_status, cudaStream_t st);
+int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, const int (&fit)[3], int* d_status,
+                    cudaStream_t st);
 size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows, int sms);
 int cache_prepare();
 

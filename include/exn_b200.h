@@ -294,9 +294,10 @@ int exn_enc_release(exn_enc* e);
  * is CUDA's default stream): no allocation, no host wait, capturable into a CUDA graph, the current
  * device left as it was.  Lengths and tables are read when the kernels run.  What the kernels find wrong
  * there (offsets that decrease or pass ROWS, lengths shorter than a sequence's rows, a page that is not
- * the pool's) they leave out, and exn_attn_sync reports it.  The calls keep nothing between them, so
+ * the pool's) they leave out, and exn_attn_sync reports it; such a sequence's rows and pages then hold
+ * anything, other sequences' are right.  The calls keep nothing between them, so
  * calls on different streams may run at once, except on the same workspace or, where one writes, on the
- * same pages. */
+ * same pages.  The same call gives the same bits again.  One thread at a time uses a handle. */
 typedef struct exn_attn exn_attn;
 
 int exn_attn_open(int device, exn_attn** out);
@@ -347,7 +348,11 @@ int exn_attn_cache_read(exn_attn* a, const exn_kv_cache* cache, int type, const 
 
 /* Attention over the cache: the rows of sequence s, its last positions, each see the positions up to
  * their own (their keys and values written before).  WORKSPACE: exn_attn_cache_workspace's bytes for these
- * ROWS and heads, 256-byte aligned, not shared by calls that may run at once (NULL when 0 bytes). */
+ * ROWS and heads, 256-byte aligned, not shared by calls that may run at once; what it holds before and
+ * after a call does not matter.  With few rows (tokens times query heads of a key/value head: up to 64 a
+ * sequence on average and 64 more) the codes are read as they are; with more, they are turned into 16 bits
+ * in the workspace once (4 * nseq * table_ld * 64 * kv_heads * 128 bytes).  Where lens[s] is less than
+ * the sequence's rows, the first rows see nothing and are 0. */
 int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int heads, const int32_t* offsets,
                           int64_t rows, const void* q, int64_t ld_q, void* out, int64_t ld_out, double scale,
                           void* workspace, size_t workspace_bytes, void* stream);

@@ -9,6 +9,13 @@ weights and A = sum_j w_j |v_j| of the same row and dim:
     sum |q k| <= scale |q| |k| stays below 31 for the rows below (|q|, |k| <= 18.5), so the weights by
     130 * 31 * 2^-24 = 2^-12 relatively; sums of weights and outputs add less than 2^-16: 2^-11.5 A;
   * an output below the type's normal range: its smallest step.
+
+Where a cache's codes are read directly, the scores' sums are exact integers and q is what is rounded, to two
+int8 numbers, q = 2^a (hi + lo / 256) with 127 2^a < 2 M for the row's largest |q| = M: an element from M / 128
+(bf16) or M / 16 (fp16) on is exact, a smaller one off by at most 2^-15 M, evenly spread.  M stays below 4.5 for
+the rows below (1.6 times that where they are spread), and of 128 normal elements fewer than 60 lie below M / 16,
+so with independent errors a score has a deviation of at most 2^-15 4.5 / sqrt(3) sqrt(60) / sqrt(128) = 2^-14.1
+and stays below 2^-11.5 at six of them: the fp32 term above covers it, its score part not being needed.
 """
 import ctypes
 import math
@@ -555,6 +562,51 @@ def test_calls_on_other_streams_and_after_slow_work(att):
     for s, (out, _, _) in zip((s1, s2), outs):
         att.sync(s.cuda_stream)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 40])
+def test_attention_over_a_cache_twice_at_once(att, tokens):
+    """The same call on two streams that wait for the same slow work, with a workspace each: both have the
+    bits of a call alone; afterwards one workspace serves calls of other sizes and the first again."""
+    heads, kv_heads, lens = 8, 2, [3000, 70, 900]
+    c = Cache(3, 47, kv_heads)
+    k, v = rows(sum(lens), kv_heads, 1, "bf16"), rows(sum(lens), kv_heads, 2, "bf16")
+    c.write(att, lens, k, v, "bf16")
+    q = rows(3 * tokens, heads, 3, "bf16")
+    want = c.attend(att, [tokens] * 3, q, heads, "bf16")
+    c.check_attend(want, [tokens] * 3, q, heads, "bf16")
+    n = att.cache_workspace(c.c, 3 * tokens, heads)
+    o, one = offsets([tokens] * 3), offsets([1, 1, 1])
+    n1 = att.cache_workspace(c.c, 3, heads)
+    spaces = [torch.zeros(max(n, n1), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    outs = [torch.zeros_like(want) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    big = torch.randn(4096, 4096, device="cuda")
+    for _ in range(4):
+        big = big @ big * 1e-3
+    ready = torch.cuda.Event()
+    ready.record()
+    for st, w, out in zip(streams, spaces, outs):
+        st.wait_event(ready)
+        for _ in range(5):
+            att.cache_attend(c.c, q.data_ptr(), out.data_ptr(), o.data_ptr(), 3 * tokens, heads, workspace=w.data_ptr(),
+                             workspace_bytes=n, stream=st.cuda_stream)
+    for st, out in zip(streams, outs):
+        att.sync(st.cuda_stream)
+        assert torch.equal(out, want)
+    small = torch.zeros(3, heads * D, dtype=torch.bfloat16, device="cuda")
+    st = streams[0].cuda_stream
+    att.cache_attend(c.c, q.data_ptr(), small.data_ptr(), one.data_ptr(), 3, heads, workspace=spaces[0].data_ptr(),
+                     workspace_bytes=n1, stream=st)
+    outs[0].zero_()
+    torch.cuda.synchronize()
+    att.cache_attend(c.c, q.data_ptr(), outs[0].data_ptr(), o.data_ptr(), 3 * tokens, heads, workspace=spaces[0].data_ptr(),
+                     workspace_bytes=n, stream=st)
+    att.sync(st)
+    assert torch.equal(outs[0], want)
+    c.dense = False
+    c.check_attend(small, [1, 1, 1], q[:3], heads, "bf16")
 
 
 # --------------------------------------------------------------------------- refusals
