@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(256) k_cache_read(const CacheArgs c, const int
 // item costs by itself.  The work of all items, laid end to end, is cut into equal parts, one a CTA, so a
 // launch is one wave whatever the lengths: a long sequence is shared by many CTAs, short ones share a CTA.
 // In a CTA one warp brings the data and the others compute: the producer finds the CTA's part of the work,
-// turns each item's rows of q into the MMA's operand and streams the spans with TMA, dealt out to the
+// turns each item's rows of q into the MMA's operand (but the first's, whose readers wait) and streams the spans with TMA, dealt out to the
 // other warps in turn, through a ring of 4 KB tiles each (K_0 V_0 K_1 ..; 128-byte swizzle, so that the
 // reads below touch every bank once); it runs ahead from one item into the next.  Each computing warp has
 // its own running maximum, sum and output, joined through shared memory at the item's end.  An item that is
@@ -363,6 +363,11 @@ __device__ __forceinline__ int count_part(unsigned long long* at, unsigned long 
   return static_cast<int>(v & 0xffffull);
 }
 
+// TX more bytes expected in the phase at hand; no arrival
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t tx) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(tx) : "memory");
+}
+
 // whether the phase of parity PARITY is complete; never waits
 __device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -407,6 +412,29 @@ struct AttendShared {
   float m[C::WARPS][C::ROWS], l[C::WARPS][C::ROWS];
   int part_len, lead, taken, abort_word;
 };
+
+// A row of q, four dims a lane, as 2^a (hi + lo / 256) into row R of segment buffer B.  By a whole warp.
+template <bool F16, int NT>
+__device__ __forceinline__ void put_query(AttendShared<NT>& sh, int b, int r, uint2 w, float scale_log2) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t mag = __vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);  // magnitudes order as their bits do
+  const float mx = unpack16<F16>(__reduce_max_sync(0xffffffffu, max(mag & 0xffffu, mag >> 16))).x;
+  const bool bad = !(mx < INFINITY);
+  const int e = scale_exponent(bad ? 0.f : mx);
+  const float inv = pow2(-e);
+  const float2 v01 = unpack16<F16>(w.x), v23 = unpack16<F16>(w.y);
+  const float v[4] = {v01.x, v01.y, v23.x, v23.y};
+  uint32_t hi[4], lo[4];  // in the low bits of floats near 1.5 * 2^23, whose unit is 1
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = v[i] * inv, h = __fadd_rd(x + 0.5f, 0x1.8p23f);  // halves up: lo = -128 there
+    hi[i] = __float_as_uint(h);
+    lo[i] = __float_as_uint(fminf(fmaf(x - (h - 0x1.8p23f), 256.f, 0x1.8p23f), 0x1.8p23f + 127.f));
+  }
+  sh.q[b][0][r][lane] = __byte_perm(__byte_perm(hi[0], hi[1], 0x0040), __byte_perm(hi[2], hi[3], 0x0040), 0x5410);
+  sh.q[b][1][r][lane] = __byte_perm(__byte_perm(lo[0], lo[1], 0x0040), __byte_perm(lo[2], lo[3], 0x0040), 0x5410);
+  if (lane == 0) sh.q_scale[b][r] = bad ? __uint_as_float(0x7fffffffu) : scale_log2 * pow2(e);  // not finite: NaN
+}
 
 // ---- the producer warp
 template <bool F16, int NT>
@@ -565,6 +593,10 @@ __device__ __forceinline__ void attend_produce(const CUtensorMap* tmK, const CUt
     }
     return r;
   };
+  // what a computing warp has to know of span SP; one that is left out lies behind every row
+  auto span_meta = [](const Ids& x, int sp) {
+    return make_float4(x.sk, x.sv, __int_as_float(x.sk < 0.f ? 0x7ffffff0 - SPAN : sp * SPAN), 0.f);
+  };
   // a segment's rows, four dims a lane
   uint2 qw[ROWS];
   auto load_q = [&](const Seg& x) {
@@ -590,45 +622,7 @@ __device__ __forceinline__ void attend_produce(const CUtensorMap* tmK, const CUt
   const int* cur_table = table;
   int cur_seen = seen;
   Ids ids = {};
-  if (cur.n) {
-    ids = fetch_ids(cur, cur_table, cur_seen, turn);
-    load_q(cur);
-  }
-  bool ok = true;
-  for (int k = 0;; ++k) {
-    const int b = k & 1;
-    ok = ok && mbar_wait_uniform(&sh.seg_empty[b], ((k >> 1) & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
-    if (!ok) cur.n = 0;
-    if (cur.n) {
-#pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const float2 v01 = unpack16<F16>(qw[r].x), v23 = unpack16<F16>(qw[r].y);
-        const float v[4] = {v01.x, v01.y, v23.x, v23.y};
-        float mx = 0.f;
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          mx = fmaxf(mx, fabsf(v[i]));
-          bad |= !(fabsf(v[i]) < INFINITY);
-        }
-        if (bad) mx = INFINITY;
-        // the bits of floats that are not negative order as integers do
-        mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
-        bad = !(mx < INFINITY);
-        const int e = scale_exponent(bad ? 0.f : mx);
-        const float inv = pow2(-e);
-        uint32_t hi = 0, lo = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = v[i] * inv, h = floorf(x + 0.5f);
-          hi |= (static_cast<uint32_t>(static_cast<int>(h)) & 0xffu) << (8 * i);
-          lo |= (static_cast<uint32_t>(min(__float2int_rn((x - h) * 256.f), 127)) & 0xffu) << (8 * i);
-        }
-        sh.q[b][0][r][lane] = hi;
-        sh.q[b][1][r][lane] = lo;
-        if (lane == 0) sh.q_scale[b][r] = bad ? __uint_as_float(0x7fffffffu) : p.scale_log2 * pow2(e);  // not finite: NaN
-      }
-    }
+  auto publish = [&](int b) {
     if (lane == 0) {
       sh.seg[b] = cur;
       sh.part_len = part_len;
@@ -636,6 +630,37 @@ __device__ __forceinline__ void attend_produce(const CUtensorMap* tmK, const CUt
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sh.seg_full[b]);
+  };
+  publish(0);  // the first segment's rows are turned into the operand by the computing warps, which wait anyway
+  if (cur.n) {
+    ids = fetch_ids(cur, cur_table, cur_seen, turn);
+    // each warp's first span: the scales may come after K's copy has begun, so its barrier's one arrival is left
+    // until they are there
+    if (lane < WARPS && turn < cur.n) {
+      const int sp = cur.sp0 + turn, row = (sp & 1) * SPAN, at = ids.pid * kv + cur.kvh;
+      uint8_t* const k0 = ring + lane * SLOTS * SPAN_BYTES;
+      mbar_expect_tx(&sh.full[lane][0], SPAN_BYTES);
+      tma_load_3d(k0, tmK, &sh.full[lane][0], 0, row, at);
+      mbar_arrive_expect_tx(&sh.full[lane][1], SPAN_BYTES);
+      tma_load_3d(k0 + SPAN_BYTES, tmV, &sh.full[lane][1], 0, row, at);
+      sh.meta[lane][0] = span_meta(ids, sp);
+      mbar_arrive(&sh.full[lane][0]);
+      slot = 2;
+      use = 1;
+      turn += WARPS;
+    }
+    ids = fetch_ids(cur, cur_table, cur_seen, turn);
+  }
+  bool ok = true;
+  for (int k = 0;; ++k) {
+    const int b = k & 1;
+    if (k > 0) ok = ok && mbar_wait_uniform(&sh.seg_empty[b], ((k >> 1) & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+    if (!ok) cur.n = 0;
+    if (cur.n && k > 0) {
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) put_query<F16, NT>(sh, b, r, qw[r], p.scale_log2);
+    }
+    if (k > 0) publish(b);
     if (!cur.n) break;
     // the next segment's rows and pages are on their way while this one's spans are dealt out
     const Seg next = advance();
@@ -655,8 +680,7 @@ __device__ __forceinline__ void attend_produce(const CUtensorMap* tmK, const CUt
       if (ready) {
         const int sp = cur.sp0 + turn;
         if (!v)
-          sh.meta[lane][use & 1] =
-              make_float4(ids.sk, ids.sv, __int_as_float(ids.sk < 0.f ? 0x7ffffff0 - SPAN : sp * SPAN), 0.f);
+          sh.meta[lane][use & 1] = span_meta(ids, sp);
         mbar_arrive_expect_tx(&sh.full[lane][slot], SPAN_BYTES);
         tma_load_3d(ring + (lane * SLOTS + slot) * SPAN_BYTES, v ? tmV : tmK, &sh.full[lane][slot], 0, (sp & 1) * SPAN,
                     ids.pid * kv + cur.kvh);
@@ -755,6 +779,17 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
     if (!ok) break;
     const int n = sh.seg[b].n, nh = sh.seg[b].nh, nrows = sh.seg[b].tok * nh, pos0 = sh.seg[b].pos0;
     if (n == 0) break;
+    if (k == 0) {
+      const int row0 = sh.seg[0].row0, head0 = sh.seg[0].head0;
+      for (int r = warp; r < ROWS; r += WARPS) {
+        uint2 w = make_uint2(0u, 0u);
+        if (r < nrows)
+          w = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + (row0 + r / nh) * p.ld_q +
+                                                   (head0 + r % nh) * 128 + 4 * lane));
+        put_query<F16, NT>(sh, 0, r, w, p.scale_log2);
+      }
+      barrier();
+    }
     // Q^T as the MMA's 32 x 8 operand, hi and lo: this thread's query row is gi (+ 8), its dims 32 ti .. + 31;
     // k-step ks multiplies dims 32 ti + 8 ks .. + 7 (which dims sit where is free as long as q and K agree)
     uint32_t qf[NT][2][8];
@@ -1040,6 +1075,17 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
     }
     barrier();
     if (sh.taken) {
+      // a row's four values at 4 (x & 31) of eight parts, on their way before they are needed
+      const auto fetch = [&](int x, int i0, float4 (&y)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (x < nrows * 32 && i0 + i < parts)
+            y[i] = __ldcg(reinterpret_cast<const float4*>(
+                              plan.part + (static_cast<long long>(part_of(i0 + i)) * ROWS + (x >> 5)) * 132) + (x & 31));
+      };
+      int x = threadIdx.x, i0 = 0;
+      float4 y[8], a = make_float4(0.f, 0.f, 0.f, 0.f);
+      fetch(x, i0, y);
       // each part's weight 2^(m - M) and each row's sum (in the join's memory), GROUP threads a row
       constexpr int GROUP = THREADS / ROWS >= 16 ? 16 : 8;
       static_assert(GROUP * ROWS <= THREADS && GROUP * ROWS % 32 == 0, "whole warps");
@@ -1070,27 +1116,27 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
         if (sub == 0) sh.l[0][row] = t;
       }
       barrier();
-      for (int x = threadIdx.x; x < nrows * 32; x += THREADS) {
-        const int row = x >> 5;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i0 = 0; i0 < parts; i0 += 8) {  // eight loads at a time
-          float4 y[8];
+      while (x < nrows * 32) {
+        const int row = x >> 5, next_i = i0 + 8 < parts ? i0 + 8 : 0, next_x = next_i ? x : x + THREADS;
+        float4 z[8];
+        fetch(next_x, next_i, z);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i0 + i < parts)
-              y[i] = __ldcg(reinterpret_cast<const float4*>(
-                                plan.part + (static_cast<long long>(part_of(i0 + i)) * ROWS + row) * 132) + (x & 31));
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i0 + i < parts) {
-              const float c = weight[(i0 + i) * ROWS + row];
-              a.x += c * y[i].x;
-              a.y += c * y[i].y;
-              a.z += c * y[i].z;
-              a.w += c * y[i].w;
-            }
+        for (int i = 0; i < 8; ++i)
+          if (i0 + i < parts) {
+            const float c = weight[(i0 + i) * ROWS + row];
+            a.x += c * y[i].x;
+            a.y += c * y[i].y;
+            a.z += c * y[i].z;
+            a.w += c * y[i].w;
+          }
+        if (next_i == 0) {
+          store(row, x, a, sh.l[0][row]);
+          a = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        store(row, x, a, sh.l[0][row]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = z[i];
+        x = next_x;
+        i0 = next_i;
       }
       barrier();  // the join's memory is free again
     }
