@@ -22,6 +22,8 @@
 // SPLIT: where there are too few items of long sequences for the SMs, a cluster of 2, 4 or 8 CTAs shares
 // an item, each a part of its keys, and joins the parts through shared memory: with row maxima m_c,
 // sums l_c and outputs o_c of the parts and M = max m_c, o = sum 2^(m_c - M) o_c / sum 2^(m_c - M) l_c.
+// When there are more items than clusters, the longest ones are shared and a cluster's CTAs take one each
+// of the others.
 // Roles, as in the single-sequence kernel of attention.cu:
 //   warp 0      finds the next item; TMA: Q_a, Q_b once an item; K_t, V_t through a ring of 4 slots, the next
 //               item's behind the last one's
@@ -56,6 +58,7 @@ constexpr int TILE_BYTES = 2 * HALF;  // 32 KB
 constexpr int SLOTS = 4;              // K_0 V_0 K_1 V_1 ... stream through 4 slots
 constexpr int OFF_QA = 0, OFF_QB = TILE_BYTES, OFF_SLOT = 2 * TILE_BYTES, OFF_BAR = (2 + SLOTS) * TILE_BYTES;
 constexpr int PK_SMEM = OFF_BAR + 512 + 1024;
+constexpr int MIN_SHARED = 1024;           // keys of an item that is worth a cluster
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 
 // kind::f16 instruction descriptor for 16-bit operands of one type (bf16 or fp16) and fp32 sums
@@ -71,7 +74,7 @@ struct Item {
   int q_start, nq, t0, tiles;  // the sequence's first query row and rows, the item's first token and tiles
   int delta, nu[2], nloads;    // token t sees keys 0 .. t + delta; units of each tile; 128-key loads
   int kvh;                     // key/value head; -1: no more items
-  int key0;                    // a cluster's CTA: its first key
+  int key0, share;             // the CTA's first key; whether the cluster's CTAs share the item
   int k_start;                 // the sequence's first key row
 };
 
@@ -191,7 +194,8 @@ __device__ __noinline__ void mend_row(const uint16_t* q, const uint16_t* k, long
 template <bool F16, bool SPLIT>
 __global__ void __launch_bounds__(PK_THREADS, 1)
     k_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-             const __grid_constant__ CUtensorMap tmV, const PackedArgs p, int tpt, int nslots, int* status) {
+             const __grid_constant__ CUtensorMap tmV, const PackedArgs p, int tpt, int nslots, int fit,
+             int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Bars* bars = reinterpret_cast<Bars*>(smem + OFF_BAR);
@@ -251,8 +255,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     return mbar_wait(bar, parity, &none, status, STATUS_TIMEOUT_ATTN, 16 * EXN_WAIT_NS);
   };
 
-  float join_m = -INFINITY, join_l = 0.f;
-  bool has_o = false;
+  bool joined = false;
   if (warp == 0) {
     // ---- the items: pairs of query tiles, times the key/value heads.  Up to 32 sequences, a lane each, go in the
     // order of their keys, the longest first, and a sequence's last tiles, which see the most, before its first: an
@@ -332,7 +335,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       }
       x.nloads = (max(x.nu[0], x.nu[1]) + 1) / 2;
       x.key0 = 0;
-      if (SPLIT) {  // this CTA's share of the 128-key loads
+      if (SPLIT && x.share) {  // this CTA's share of the 128-key loads
         const int l0 = x.nloads * part / parts, l1 = x.nloads * (part + 1) / parts;
         x.key0 = l0 * TILE;
         x.nloads = l1 - l0;
@@ -378,7 +381,21 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       tma_prefetch(&tmV);
     }
     Item cur;
-    if (!find(static_cast<int>(blockIdx.x) / parts, cur)) next_item(cur);
+    int index = static_cast<int>(blockIdx.x);
+    cur.share = 0;
+    if (SPLIT) {
+      // The first SHARED items have a cluster each, the others a CTA: so many that all clusters run at once
+      index /= parts;
+      int shared = nslots * p.kv_heads;
+      if (sorted) {
+        const int items = p.kv_heads * static_cast<int>(__reduce_add_sync(0xffffffffu, pairs));
+        const int lengthy = p.kv_heads * static_cast<int>(__reduce_add_sync(0xffffffffu, nk >= MIN_SHARED ? pairs : 0));
+        shared = min(items <= fit ? items : max(parts * fit - items, 0) / (parts - 1), lengthy);
+      }
+      cur.share = index < shared;
+      if (!cur.share) index = shared + (index - shared) * parts + part;
+    }
+    if (!find(index, cur)) next_item(cur);
     uint32_t q_count[2] = {0, 0}, loads = 0;  // so far
     for (uint32_t k = 0;; ++k) {
       const int ib = k & 1;
@@ -625,13 +642,67 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         }
       }
       units += n;
-      if (SPLIT) {  // the join is behind the roles
+      if (SPLIT && it.share) {
+        // ---- the join of a cluster's parts.  Every CTA owns PER rows: all send their share of O (fp32) and (m, l)
+        // there, over Q's and the ring's memory (16 bytes i of the owner's row j at i ^ (j % 32)), and the owner joins
+        // them, a warp a row.
         if (n > 0) ok = ok && mbar_wait_uniform(&bars->o_full[x], 0, abort_flag, status, STATUS_TIMEOUT_ATTN);
         tc_fence_after();
-        join_m = m;
-        join_l = lsum;
-        has_o = n > 0 && ok;
-        continue;
+        cluster_sync();  // every CTA's MMAs are done
+        const int per = 2 * TILE / parts;
+        float2* const ml = reinterpret_cast<float2*>(smem + OFF_SLOT + 2 * TILE_BYTES);
+        {
+          const int row = x * TILE + r, j = row % per, owner = row / per;
+          const uint32_t dst = mapa_shared(smem + (part * per + j) * 512, owner);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t rr[32];
+            if (n > 0 && ok) {
+              tmem_ld32(o_addr + c * 32, rr);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) rr[i] = 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) st_cluster_v4(dst + (((c * 8 + i) ^ (j & 31)) << 4), rr + 4 * i);
+          }
+          st_cluster_f2(mapa_shared(ml + part * per + j, owner), m, lsum);
+        }
+        cluster_sync();
+#pragma unroll 1
+        for (int j = warp - 3; j < per; j += 8) {
+          const int row = part * per + j, y = row / TILE, rj = row - y * TILE, tj = rj / g, token = it.t0 + y * tpt + tj;
+          if (y >= tiles || tj >= tpt || token >= nq) continue;
+          float mx = -INFINITY, l = 0.f;
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int c = 0; c < parts; ++c) mx = fmaxf(mx, ml[c * per + j].x);
+          const float mu = mx == -INFINITY ? 0.f : mx;
+          for (int c = 0; c < parts; ++c) {
+            const float2 a = ml[c * per + j];
+            const float4 z = reinterpret_cast<const float4*>(smem + (c * per + j) * 512)[lane ^ (j & 31)];
+            const float w = fast_exp2(a.x - mu);
+            l += w * a.y;
+            o.x += w * z.x;
+            o.y += w * z.y;
+            o.z += w * z.z;
+            o.w += w * z.w;
+          }
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+          const int head = kvh * g + rj - tj * g;
+          uint16_t* const dst = out + static_cast<long long>(q_start + token) * p.ld_out + head * 128;
+          reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack16<F16>(o.x, o.y), pack16<F16>(o.z, o.w));
+          if (__any_sync(0xffffffffu, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)))) {
+            const long long seen = min(nq, it.t0 + (y + 1) * tpt) + delta;  // by the tile's last row
+            const long long end = min((seen + UNIT - 1) / UNIT * UNIT, p.kv_rows - k_start), k0 = k_start;
+            mend_row<F16>(static_cast<const uint16_t*>(p.q) + static_cast<long long>(q_start + token) * p.ld_q + head * 128,
+                          static_cast<const uint16_t*>(p.k) + k0 * p.ld_k + kvh * 128, p.ld_k,
+                          static_cast<const uint16_t*>(p.v) + k0 * p.ld_v + kvh * 128, p.ld_v, token + delta,
+                          static_cast<int>(end) - 1, p.scale_log2, dst);
+          }
+        }
+        joined = true;
+        break;  // a cluster has one item
       }
       const int head = kvh * g + r - tok * g;
       uint16_t* dst = out + static_cast<long long>(q_start + t) * p.ld_out + head * 128;
@@ -686,73 +757,14 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       }
     }
   }
+  if (SPLIT && !joined) {  // the join's barriers are all threads', whatever ended their work
+    __syncwarp();
+    cluster_sync();
+    cluster_sync();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // ---- the join of a cluster's parts.  Every CTA owns PER rows: all send their share of O (fp32) and (m, l) there,
-  // over Q's and the ring's memory (16 bytes i of the owner's row j at i ^ (j % 32)), and the owner joins them, a
-  // warp a row.
-  const Item& it = bars->item[0];  // all the cluster's CTAs have the same item, or none
-  if (SPLIT) {
-    const int per = 2 * TILE / parts;
-    float2* const ml = reinterpret_cast<float2*>(smem + OFF_SLOT + 2 * TILE_BYTES);
-    cluster_sync();  // every CTA's MMAs are done
-    if (warp >= 3 && it.kvh >= 0) {
-      const int x = (warp - 3) >> 2, row = x * TILE + (warp & 3) * 32 + lane, j = row % per, owner = row / per;
-      const uint32_t o_addr = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 256 + x * 128;
-      const uint32_t dst = mapa_shared(smem + (part * per + j) * 512, owner);
-      const int swz = j & 31;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t rr[32];
-        if (__all_sync(0xffffffffu, has_o)) {
-          tmem_ld32(o_addr + c * 32, rr);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) rr[i] = 0u;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) st_cluster_v4(dst + (((c * 8 + i) ^ swz) << 4), rr + 4 * i);
-      }
-      st_cluster_f2(mapa_shared(ml + part * per + j, owner), join_m, join_l);
-    }
-    cluster_sync();
-    if (warp >= 3 && it.kvh >= 0) {
-#pragma unroll 1
-      for (int j = warp - 3; j < per; j += 8) {
-        const int row = part * per + j, x = row / TILE, r = row - x * TILE, tok = r / g, t = it.t0 + x * tpt + tok;
-        if (x >= it.tiles || tok >= tpt || t >= it.nq) continue;
-        float m = -INFINITY, l = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int c = 0; c < parts; ++c) m = fmaxf(m, ml[c * per + j].x);
-        const float mu = m == -INFINITY ? 0.f : m;
-        for (int c = 0; c < parts; ++c) {
-          const float2 y = ml[c * per + j];
-          const float4 z = reinterpret_cast<const float4*>(smem + (c * per + j) * 512)[lane ^ (j & 31)];
-          const float w = fast_exp2(y.x - mu);
-          l += w * y.y;
-          o.x += w * z.x;
-          o.y += w * z.y;
-          o.z += w * z.z;
-          o.w += w * z.w;
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-        const int head = it.kvh * g + r - tok * g;
-        uint16_t* const dst = out + static_cast<long long>(it.q_start + t) * p.ld_out + head * 128;
-        reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack16<F16>(o.x, o.y), pack16<F16>(o.z, o.w));
-        if (__any_sync(0xffffffffu, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)))) {
-          const int lim = t + it.delta, seen = min(it.nq, it.t0 + (x + 1) * tpt) + it.delta;  // by the tile's last row
-          const long long end = min((seen + static_cast<long long>(UNIT) - 1) / UNIT * UNIT, p.kv_rows - it.k_start);
-          const long long k0 = it.k_start;
-          mend_row<F16>(static_cast<const uint16_t*>(p.q) + static_cast<long long>(it.q_start + t) * p.ld_q + head * 128,
-                        static_cast<const uint16_t*>(p.k) + k0 * p.ld_k + it.kvh * 128, p.ld_k,
-                        static_cast<const uint16_t*>(p.v) + k0 * p.ld_v + it.kvh * 128, p.ld_v, lim,
-                        static_cast<int>(end) - 1, p.scale_log2, dst);
-        }
-      }
-    }
-  }
   if (warp == 1) {
     __syncwarp();
     tmem_dealloc(tmem, 512);
@@ -813,18 +825,22 @@ int packed_launch(const PackedArgs& a, int* d_status, cudaStream_t st) {
     return -4;
   const long long nslots = (a.rows - 1) / (2 * tpt) + a.nseq, items = nslots * a.kv_heads;  // at most
   if (items > 0x7fffffffll) return -1;
-  // CTAs an item.  A cluster's launch and join cost about 10 us, so it has to have keys enough to share, and all
-  // clusters run at once (74 of 2, 33 of 4, 15 of 8).  us at 1, 2, 4 and 8 CTAs an item (32 heads over 8, bf16):
+  // CTAs a cluster.  Its launch and join cost about 10 us, so it has to have keys enough to share, and all clusters
+  // run at once (74 of 2, 33 of 4, 15 of 8).  us at 1, 2, 4 and 8 CTAs an item (32 heads over 8, bf16):
   //   64 rows (8 items)    over  1024 keys:  22   25   20   21    over 16384 keys: 249  138   76   49
   //   192 rows (32 items)  over  1024 keys:  23   26   21   38    over  8192 keys: 128   78   48   65
   //   512 rows (72 items)  over  1024 keys:  23   26   42   87    over  8192 keys: 130   80   96  153
+  // Up to twice the clusters of 2, some items are shared; with one sequence, whose items are alike, that gains
+  // nothing (1024 rows over 1100 keys: 24 us alone, 30 so), with several it does when their keys differ (300, 77,
+  // 512 and 9 rows over 4100, 900, 513 and 5 keys, 28 heads over 4: 69 us alone, 51 so).
   const long long keys = a.kv_rows / a.nseq;
-  const int parts = keys >= 1024 && items <= a.fit[2] ? 8 : keys >= 1024 && items <= a.fit[1] ? 4
-                    : keys >= 2048 && items <= a.fit[0] ? 2 : 1;
-  const PackedLaunch l(static_cast<unsigned>(items), parts, st);
+  const int parts = keys < MIN_SHARED ? 1 : items <= a.fit[2] ? 8 : items <= a.fit[1] ? 4
+                    : keys >= 2048 && items <= a.fit[0] ? 2 : a.nseq > 1 && a.nseq <= 32 && items <= 2 * a.fit[0] ? 2 : 1;
+  const int fit = parts > 1 ? a.fit[parts == 8 ? 2 : parts == 4 ? 1 : 0] : 0;
+  const PackedLaunch l(static_cast<unsigned>(parts > 1 && items > fit ? fit : items), parts, st);
   auto* const kernel = parts > 1 ? (a.f16 ? k_packed<true, true> : k_packed<false, true>)
                                  : (a.f16 ? k_packed<true, false> : k_packed<false, false>);
-  return static_cast<int>(cudaLaunchKernelEx(&l.cfg, kernel, tq, tk, tv, a, tpt, static_cast<int>(nslots), d_status));
+  return static_cast<int>(cudaLaunchKernelEx(&l.cfg, kernel, tq, tk, tv, a, tpt, static_cast<int>(nslots), fit, d_status));
 }
 
 }  // namespace exn

@@ -220,10 +220,12 @@ def test_packed_deterministic_and_independent_of_the_packing(att):
 @pytest.mark.parametrize("t", ["bf16", "fp16"])
 @pytest.mark.parametrize("heads,kv_heads", [(8, 2), (28, 4), (5, 1), (16, 16)])
 @pytest.mark.parametrize("nq,nk", [([64], [5000]), ([1], [1024]), ([70, 3, 40], [4200, 0, 1500]), ([129, 0], [2049, 63]),
-                                   ([300, 77], [4100, 900])])
+                                   ([300, 77], [4100, 900]), ([20, 290, 1, 33], [1500, 300, 9, 2500]),
+                                   ([200] * 4, [5000, 1030, 600, 1])])
 def test_packed_few_rows_over_long_keys(att, heads, kv_heads, t, nq, nk):
     """Few work items of long sequences, whose keys several blocks share: from a share of one load to many,
-    a last share that only the item's later rows see, a sequence without keys beside long ones."""
+    a last share that only the item's later rows see, a sequence without keys beside long ones; more items
+    than clusters, of which the long ones are shared."""
     q, k, v = rows(sum(nq), heads, 1, t), rows(sum(nk), kv_heads, 2, t), rows(sum(nk), kv_heads, 3, t)
     out = run_packed(att, q, k, v, nq, heads, kv_heads, t, nk=nk)
     check_packed(out, q, k, v, nq, heads, kv_heads, t, nk=nk)
