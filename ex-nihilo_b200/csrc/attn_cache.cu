@@ -1208,8 +1208,13 @@ static bool dense_path(const CacheArgs& c, int heads, long long rows) {
 }
 static long long dense_rows(const CacheArgs& c) { return static_cast<long long>(c.nseq) * c.table_ld * kPage; }
 
-// the cut of the direct path's work: 8 or 16 query rows a tile, 16 when the sequences' rows (on average)
-// need more than 8; a wave of CTAs
+// the cut of the direct path's work: a wave of CTAs, tiles of 8 or 16 query rows.  us with tiles of 8 / 16
+// (bf16; the codes are read again for every tile):
+//   rows a sequence                            4             8            12            32
+//   1 sequence of 64000, 32 heads over 8   34 / 41       38 / 43       49 / 43       80 / 68
+//   8 of 8000, 32 over 8                   32 / 40       33 / 41       50 / 42       92 / 69
+//   64 of 4000, 32 over 8                  96 / 123      97 / 126     175 / 129     334 / 235
+// so 16 when the sequences' rows (on average) need more than 8.
 static AttendPlan attend_plan(const CacheArgs& c, int heads, long long rows, int sms, void* ws) {
   AttendPlan p;
   const int g = heads / c.kv_heads;
@@ -1229,10 +1234,12 @@ static AttendPlan attend_plan(const CacheArgs& c, int heads, long long rows, int
   p.count = reinterpret_cast<unsigned long long*>(p.part + 2ll * p.ctas * 8 * nt * 132);
   return p;
 }
+// enough for ROWS and for any fewer
 size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows, int sms) {
-  if (dense_path(c, heads, rows)) return static_cast<size_t>(dense_rows(c)) * c.kv_heads * 128 * 2 * 2;
-  const AttendPlan p = attend_plan(c, heads, rows, sms, nullptr);
-  return static_cast<size_t>(p.ctas) * (2 * 16 * 132 * 4 + 8);
+  static_assert(AttendCfg<1>::CTAS >= AttendCfg<2>::CTAS, "the most CTAs, parts of the most rows");
+  const size_t codes = static_cast<size_t>(sms) * AttendCfg<1>::CTAS * (2 * AttendCfg<2>::ROWS * 132 * 4 + 8);
+  const size_t dense = static_cast<size_t>(dense_rows(c)) * c.kv_heads * 128 * 2 * 2;
+  return dense_path(c, heads, rows) && dense > codes ? dense : codes;
 }
 
 static int attend_launch(const CacheAttnArgs& a, void* ws, int sms, int* d_status, cudaStream_t st) {

@@ -244,7 +244,8 @@ int exn_enc_states_device(exn_enc* e, const int32_t* ids, int n, const int32_t* 
 /* Several prompts in one pass, for the pictures of exn_generate_batch / exn_generate_device: IDS holds
  * COUNTS[0] token ids of the first prompt, then COUNTS[1] of the second, .. (32768 in all; a count may
  * be 0), POSITIONS (or NULL: (i, i, i) within each prompt) and STATES likewise.  Every prompt's states are those
- * of a pass of its own; the weights are read once for all of them. */
+ * of a pass of its own but for rounding (the products' sums are cut by the pass's size); the weights are
+ * read once for all of them. */
 int exn_enc_states_packed(exn_enc* e, const int32_t* ids, int nseq, const int32_t* counts, const int32_t* positions,
                           float* states);
 
@@ -348,7 +349,7 @@ int exn_attn_cache_read(exn_attn* a, const exn_kv_cache* cache, int type, const 
 
 /* Attention over the cache: the rows of sequence s, its last positions, each see the positions up to
  * their own (their keys and values written before).  WORKSPACE: exn_attn_cache_workspace's bytes for these
- * ROWS and heads, 256-byte aligned, not shared by calls that may run at once; what it holds before and
+ * ROWS (or more) and heads, 256-byte aligned, not shared by calls that may run at once; what it holds before and
  * after a call does not matter.  With few rows (tokens times query heads of a key/value head: up to 64 a
  * sequence on average and 64 more) the codes are read as they are; with more, they are turned into 16 bits
  * in the workspace once (4 * nseq * table_ld * 64 * kv_heads * 128 bytes).  Where lens[s] is less than

@@ -331,7 +331,9 @@ class Cache:
         att.cache_attend(self.c, q.data_ptr(), out.data_ptr(), o.data_ptr(), q.shape[0], heads, dtype=GGML[t],
                          ld_q=q.stride(0), ld_out=out.stride(0), workspace=w.data_ptr(), workspace_bytes=n, stream=stream)
         att.sync(stream)
-        self.dense = n == self.c.nseq * self.c.table_ld * 64 * self.kv * D * 2 * 2  # keys and values in 16 bits
+        self.dense = q.shape[0] * (heads // self.kv) > 64 * (self.c.nseq + 1)  # keys and values in 16 bits
+        assert n >= att.cache_workspace(self.c, 1, heads)
+        assert not self.dense or n >= self.c.nseq * self.c.table_ld * 64 * self.kv * D * 2 * 2
         return out
 
     def check_attend(self, out, counts, q, heads, t):
