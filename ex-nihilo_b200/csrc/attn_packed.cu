@@ -344,12 +344,10 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       }
       return true;
     };
-    // The next item is asked for late: near the end of the item at hand, and not in the kernel's first
-    // microseconds, when the CTAs that have not started are still finding SMs of their own.
+    // The next item is asked for late, near the end of the item at hand: it may be one that would soon have found
+    // an SM of its own.
     uint32_t claims = 0;
     bool ok = true, asked = false, ended = SPLIT;
-    const uint64_t t_start = globaltimer();
-    auto settled = [&] { return __any_sync(0xffffffffu, globaltimer() - t_start > 3000); };
     auto ask = [&] {
       if (lane == 0) claim_request(&bars->claim, &bars->claim_full);
       asked = true;
@@ -357,10 +355,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     auto next_item = [&](Item& x) {  // kvh -1: no more
       x.kvh = -1;
       while (!ended && ok) {
-        if (!asked) {
-          while (!settled()) __nanosleep(100);
-          ask();
-        }
+        if (!asked) ask();
         if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->claim_full, claims & 1) : true, 0)) {
           ok = false;
           return;
@@ -425,7 +420,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         }
       Item next;
       for (int t = 0; t < 2 * cur.nloads; ++t) {
-        if (t >= 2 * cur.nloads - 8 && !asked && !ended && settled()) ask();
+        if (t >= 2 * cur.nloads - 8 && !asked && !ended) ask();
         if (!ok) continue;
         const uint32_t sl = loads % SLOTS;
         ok = mbar_wait_warp(&bars->slot_empty[sl], ((loads / SLOTS) & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
@@ -612,18 +607,20 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
             }
           }
         }
+        {  // log2 of P, before the turn: what is left for it is the exponentials
+          const uint64_t nm2 = f2(nm, nm);
+#pragma unroll
+          for (int i = 0; i < UNIT; i += 2) f2_split(ffma2(f2(s[i], s[i + 1]), sc2, nm2), s[i], s[i + 1]);
+        }
         if (u < turns) asm volatile("bar.sync %0, 64;" ::"r"(my_turn) : "memory");
         uint32_t pk[UNIT / 2];  // P as 16-bit pairs: key 2c and 2c+1 in column c
         if (ok) {
-          const uint64_t nm2 = f2(nm, nm);
           uint64_t ps2[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
           for (int c8 = 0; c8 < UNIT / 8; ++c8) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float x0, x1;
-              f2_split(ffma2(f2(s[c8 * 8 + 2 * i], s[c8 * 8 + 2 * i + 1]), sc2, nm2), x0, x1);
-              const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+              const float e0 = fast_exp2(s[c8 * 8 + 2 * i]), e1 = fast_exp2(s[c8 * 8 + 2 * i + 1]);
               ps2[i] = fadd2(ps2[i], f2(e0, e1));
               pk[c8 * 4 + i] = pack16<F16>(e0, e1);
             }
