@@ -289,7 +289,7 @@ int exn_enc_release(exn_enc* e);
  * its heads side by side; ld a multiple of 8 (0: the rows are contiguous), bases 16-byte aligned.
  * OFFSETS (int32, nseq + 1, on the device, not decreasing, from 0) says which rows are whose: sequence
  * s has rows OFFSETS[s] .. OFFSETS[s + 1] - 1, possibly none; rows from OFFSETS[nseq] on, up to ROWS,
- * are left as they are.  SCALE multiplies the scores (0: 1 / sqrt(128)).
+ * are left as they are.  SCALE multiplies the scores (0: 1 / sqrt(128)).  Outputs overlap no input.
  *
  * The calls check what the host can see and queue kernels on STREAM (a cudaStream_t of the device; NULL
  * is CUDA's default stream): no allocation, no host wait, capturable into a CUDA graph, the current

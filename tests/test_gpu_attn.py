@@ -257,6 +257,44 @@ def test_packed_shared_keys_that_are_not_finite(att, t, value):
         assert torch.isnan(out[:70, :4 * D]).all()
 
 
+@pytest.mark.parametrize("nseq", [33, 70, 1100])
+def test_packed_many_sequences(att, nseq):
+    """More sequences than a warp has lanes, empty ones among them, with rows of their own and as the last
+    rows of longer ones."""
+    heads, kv_heads = 4, 2
+    nq = [(7 * i) % 11 * (i % 3 > 0) + (40 if i % 29 == 0 else 0) for i in range(nseq)]
+    for nk in (nq, [n + i % 5 for i, n in enumerate(nq)]):
+        q, k, v = rows(sum(nq), heads, 1, "bf16"), rows(sum(nk), kv_heads, 2, "bf16"), rows(sum(nk), kv_heads, 3, "bf16")
+        out = run_packed(att, q, k, v, nq, heads, kv_heads, "bf16", nk=nk)
+        check_packed(out, q, k, v, nq, heads, kv_heads, "bf16", nk=nk)
+
+
+def test_packed_captured_with_shared_items(att):
+    """Calls whose blocks share items, captured one after another and replayed with other inputs."""
+    heads, kv_heads = 8, 2
+    sets = []
+    for nq, nk in (([64], [5000]), ([30, 70], [1100, 3000]), ([300, 77, 20, 5], [4100, 900, 1500, 200])):
+        q, k, v = rows(sum(nq), heads, 1, "bf16"), rows(sum(nk), kv_heads, 2, "bf16"), rows(sum(nk), kv_heads, 3, "bf16")
+        sets.append((nq, nk, q, k, v, torch.empty_like(q), offsets(nq), offsets(nk)))
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        st = torch.cuda.current_stream().cuda_stream
+        for nq, nk, q, k, v, out, qo, ko in sets:
+            att.packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), qo.data_ptr(), len(nq), sum(nq), heads,
+                       kv_heads, kv_offsets=ko.data_ptr(), kv_rows=sum(nk), stream=st)
+    for seed in (5, 6):
+        for nq, nk, q, k, v, _, _, _ in sets:
+            q.copy_(rows(sum(nq), heads, seed, "bf16"))
+            v.copy_(rows(sum(nk), kv_heads, seed + 10, "bf16"))
+        g.replay()
+        g.replay()
+        torch.cuda.synchronize()
+        att.sync()
+        for nq, nk, q, k, v, out, _, _ in sets:
+            check_packed(out, q, k, v, nq, heads, kv_heads, "bf16", nk=nk)
+
+
 # --------------------------------------------------------------------------- the cache
 
 
@@ -611,6 +649,40 @@ def test_attention_over_a_cache_twice_at_once(att, tokens):
     assert torch.equal(outs[0], want)
     c.dense = False
     c.check_attend(small, [1, 1, 1], q[:3], heads, "bf16")
+
+
+@pytest.mark.parametrize("nseq", [70, 300])
+def test_cache_of_many_sequences(att, nseq):
+    """More sequences than lanes, and than a block's threads: written, read and attended, some with nothing
+    new, some without any position."""
+    heads, kv_heads = 4, 2
+    c = Cache(nseq, 2, kv_heads)
+    lens = [(13 * i) % 127 * (i % 7 > 0) for i in range(nseq)]
+    k, v = rows(sum(lens), kv_heads, 1, "bf16"), rows(sum(lens), kv_heads, 2, "bf16")
+    c.write(att, lens, k, v, "bf16")
+    new = [i % 2 for i in range(nseq)]
+    k, v, q = rows(sum(new), kv_heads, 3, "bf16"), rows(sum(new), kv_heads, 4, "bf16"), rows(sum(new), heads, 5, "bf16")
+    c.write(att, new, k, v, "bf16")
+    out = c.attend(att, new, q, heads, "bf16")
+    c.check_attend(out, new, q, heads, "bf16")
+    total = [a + b for a, b in zip(lens, new)]
+    got_k, got_v = c.read(att, total, "bf16")
+    assert torch.equal(got_k.double(), c.expect("k", total).flatten(1))
+    assert torch.equal(got_v.double(), c.expect("v", total).flatten(1))
+
+
+@pytest.mark.parametrize("extra", [2, 300])
+def test_rows_before_the_first_position_are_zero(att, extra):
+    """More rows than a sequence has positions: the first ones see nothing and are 0, by either path."""
+    heads, kv_heads, lens = 4, 2, [100, 0, 3]
+    c = Cache(3, 2, kv_heads)
+    k, v = rows(103, kv_heads, 1, "bf16"), rows(103, kv_heads, 2, "bf16")
+    c.write(att, lens, k, v, "bf16")
+    counts = [100 + extra, 2, 3 + extra]
+    q = rows(sum(counts), heads, 3, "bf16")
+    out = c.attend(att, counts, q, heads, "bf16")
+    c.check_attend(out, counts, q, heads, "bf16")
+    assert (out[:extra] == 0).all() and (out[100 + extra:102 + extra] == 0).all()
 
 
 # --------------------------------------------------------------------------- refusals
