@@ -191,6 +191,25 @@ __device__ __noinline__ void mend_row(const uint16_t* q, const uint16_t* k, long
       make_uint2(pack16<F16>(o[0] * inv, o[1] * inv), pack16<F16>(o[2] * inv, o[3] * inv));
 }
 
+// 32 bytes at a 32-byte boundary
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// the sum of X over the lanes before this one
+__device__ __forceinline__ int warp_before(int x) {
+  const int lane = threadIdx.x & 31;
+  int sum = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += y;
+  }
+  return sum - x;
+}
+
 template <bool F16, bool SPLIT>
 __global__ void __launch_bounds__(PK_THREADS, 1)
     k_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -257,70 +276,75 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
 
   bool joined = false;
   if (warp == 0) {
-    // ---- the items: pairs of query tiles, times the key/value heads.  Up to 32 sequences, a lane each, go in the
-    // order of their keys, the longest first, and a sequence's last tiles, which see the most, before its first: an
-    // item that starts late is then short.  (1024 rows over 5555 keys, 300 over 300 and 512 over 8192, 32 heads over
-    // 8: 160 us in that order, 200 as below.)  Of more sequences, s owns the slots from floor(start_s / pair) + s
-    // on; the distance to the next one's first slot is at least ceil(length / pair).  Either way the host knows a
-    // bound of the count of slots without the lengths.
+    // ---- the items: pairs of query tiles, times the key/value heads.  A lane has a run of the sequences and knows
+    // how many items come before it.  Up to 32 sequences, a lane each, go in the order of their keys, the longest
+    // first, and a sequence's last tiles, which see the most, before its first: an item that starts late is then
+    // short (1024 rows over 5555 keys, 300 over 300 and 512 over 8192, 32 heads over 8: 160 us so, 200 in their
+    // own order).  The host knows a bound of the count without the lengths.
     const int pair = 2 * tpt;
-    int q0 = 0, q1 = 0, k0 = 0, nk = 0, pairs = 0, first = 0;  // a sequence's rows, keys, items and its first one's place
+    struct Sequence {
+      int q0, q1, k0, nk, pairs;  // rows, keys, items a head
+    };
     auto read = [&](int s) {
-      q0 = p.q_offsets[s];
-      q1 = p.q_offsets[s + 1];
+      Sequence x;
+      x.q0 = p.q_offsets[s];
+      x.q1 = p.q_offsets[s + 1];
       long long start;
       if (p.kv_lens) {
         start = p.kv_stride * s;
-        nk = p.kv_lens[s];
+        x.nk = p.kv_lens[s];
       } else {
         start = p.kv_offsets[s];
-        nk = p.kv_offsets[s + 1] - static_cast<int>(start);
+        x.nk = p.kv_offsets[s + 1] - static_cast<int>(start);
       }
-      pairs = q0 < 0 || q1 < q0 || q1 > p.rows ? 0 : (q1 - q0 + pair - 1) / pair;
-      if (pairs && (start < 0 || nk < 0 || start + nk > p.kv_rows)) {
+      x.pairs = x.q0 < 0 || x.q1 < x.q0 || x.q1 > p.rows ? 0 : (x.q1 - x.q0 + pair - 1) / pair;
+      if (x.pairs && (start < 0 || x.nk < 0 || start + x.nk > p.kv_rows)) {
         atomicOr(status, STATUS_BAD_ARG);
-        pairs = 0;
+        x.pairs = 0;
       }
-      k0 = static_cast<int>(start);
+      x.k0 = static_cast<int>(start);
+      return x;
     };
-    const bool sorted = p.nseq <= 32;
+    const int run = (p.nseq + 31) / 32;
+    const bool sorted = run == 1;
+    Sequence mine = {0, 0, 0, 0, 0};
+    int pairs = 0, first = 0;  // of the lane's run: its items a head, those before it
     if (sorted) {
-      if (lane < p.nseq) read(lane);
+      if (lane < p.nseq) mine = read(lane);
+      pairs = mine.pairs;
       for (int j = 0; j < p.nseq; ++j) {
-        const int other = __shfl_sync(0xffffffffu, nk, j), n = __shfl_sync(0xffffffffu, pairs, j);
-        if (other > nk || (other == nk && j < lane)) first += n;
+        const int other = __shfl_sync(0xffffffffu, mine.nk, j), n = __shfl_sync(0xffffffffu, pairs, j);
+        if (other > mine.nk || (other == mine.nk && j < lane)) first += n;
       }
+    } else {
+      for (int s = lane * run; s < min(p.nseq, lane * run + run); ++s) pairs += read(s).pairs;
+      first = warp_before(pairs);
     }
-    auto find = [&](int index, Item& x) -> bool {  // by the whole warp; false: nothing at this slot
-      int i, a, b, from, keys;
-      if (sorted) {
-        const int at = index / p.kv_heads - first;
-        const unsigned owner = __ballot_sync(0xffffffffu, at >= 0 && at < pairs);
-        if (!owner) return false;
-        const int src = __ffs(owner) - 1;
-        i = __shfl_sync(0xffffffffu, pairs - 1 - at, src);
-        a = __shfl_sync(0xffffffffu, q0, src);
-        b = __shfl_sync(0xffffffffu, q1, src);
-        from = __shfl_sync(0xffffffffu, k0, src);
-        keys = __shfl_sync(0xffffffffu, nk, src);
-      } else {
-        const int sl = nslots - 1 - index / p.kv_heads;
-        int lo = 0, hi = p.nseq;  // the last sequence that owns slots up to SL, 32 probes a step
-        while (hi - lo > 1) {
-          const int step = (hi - lo + 31) / 32, s = lo + lane * step;
-          const bool below = s < hi && p.q_offsets[s] / pair + s <= sl;
-          const unsigned m = __ballot_sync(0xffffffffu, below) | 1u;
-          lo += (31 - __clz(m)) * step;
-          hi = min(hi, lo + step);
+    auto find = [&](int index, Item& x) -> bool {  // by the whole warp; false: no such item
+      int at = index / p.kv_heads - first;
+      unsigned owner = __ballot_sync(0xffffffffu, at >= 0 && at < pairs);
+      if (!owner) return false;
+      int src = __ffs(owner) - 1;
+      Sequence mine_now = mine;
+      if (!sorted) {  // the owner's run, 32 sequences at a time
+        at = __shfl_sync(0xffffffffu, at, src);
+        const int end = min(p.nseq, src * run + run);
+        for (int s0 = src * run;; s0 += 32) {
+          if (s0 >= end) return false;  // not before the offsets change under the kernel
+          mine_now = s0 + lane < end ? read(s0 + lane) : Sequence{0, 0, 0, 0, 0};
+          const int before = warp_before(mine_now.pairs);
+          owner = __ballot_sync(0xffffffffu, at >= before && at < before + mine_now.pairs);
+          if (owner) {
+            at -= before;
+            break;
+          }
+          at -= __shfl_sync(0xffffffffu, before + mine_now.pairs, 31);
         }
-        read(lo);
-        i = sl - (q0 / pair + lo);
-        if (i < 0 || i >= pairs) return false;
-        a = q0;
-        b = q1;
-        from = k0;
-        keys = nk;
+        src = __ffs(owner) - 1;
       }
+      const int i = __shfl_sync(0xffffffffu, mine_now.pairs - 1 - at, src), a = __shfl_sync(0xffffffffu, mine_now.q0, src),
+                b = __shfl_sync(0xffffffffu, mine_now.q1, src), from = __shfl_sync(0xffffffffu, mine_now.k0, src),
+                keys = __shfl_sync(0xffffffffu, mine_now.nk, src);
       x.t0 = i * pair;
       x.q_start = a;
       x.nq = b - a;
@@ -384,7 +408,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       int shared = nslots * p.kv_heads;
       if (sorted) {
         const int items = p.kv_heads * static_cast<int>(__reduce_add_sync(0xffffffffu, pairs));
-        const int lengthy = p.kv_heads * static_cast<int>(__reduce_add_sync(0xffffffffu, nk >= MIN_SHARED ? pairs : 0));
+        const int lengthy = p.kv_heads * static_cast<int>(__reduce_add_sync(0xffffffffu, mine.nk >= MIN_SHARED ? pairs : 0));
         shared = min(items <= fit ? items : max(parts * fit - items, 0) / (parts - 1), lengthy);
       }
       cur.share = index < shared;
@@ -542,6 +566,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     const uint32_t other_turn = (x ? 1u : 5u) + static_cast<uint32_t>(wq);
     uint32_t units = 0, o_count = 0;  // of the items before
     bool ok = true;
+    const bool wide = ((reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(2 * p.ld_out)) & 31) == 0;
     for (uint32_t k = 0;; ++k) {
       const int ib = k & 1;
       if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->item_full[ib], (k >> 1) & 1) : true, 0)) break;
@@ -722,11 +747,18 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
               finite = fmaf(o[i], 0.f, finite);
             }
             if (live) {
-              uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+              uint32_t w[16];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                d4[i] = make_uint4(pack16<F16>(o[8 * i], o[8 * i + 1]), pack16<F16>(o[8 * i + 2], o[8 * i + 3]),
-                                   pack16<F16>(o[8 * i + 4], o[8 * i + 5]), pack16<F16>(o[8 * i + 6], o[8 * i + 7]));
+              for (int i = 0; i < 16; ++i) w[i] = pack16<F16>(o[2 * i], o[2 * i + 1]);
+              // a row a lane: half the lines of 16-byte stores (30 sequences of 300: 58.3 us, 62.1)
+              if (wide) {
+                st_global_32(dst + c * 32, w);
+                st_global_32(dst + c * 32 + 16, w + 8);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  reinterpret_cast<uint4*>(dst + c * 32)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+              }
             }
           }
           tc_fence_before();  // O is read before the next item's first P lets an MMA write it
