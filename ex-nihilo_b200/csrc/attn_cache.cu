@@ -89,7 +89,7 @@ __device__ __forceinline__ void find_page(const int* offsets, const int* lens, i
 
 // ---- write: one block = one page touched by the call's rows, one key/value head; threads 0..127 take
 // K, 128..255 V, 16 threads a row of 128 values.  Long prompts are bound by the bytes, 2 in and 1 out a
-// value; single tokens by the chain of dependent loads (offsets and lengths; the rows and the table's
+// value (6360 rows of 8 heads: 8.3 us, 4.7 TB/s); single tokens (64: 5.0 us) by the chain of dependent loads (offsets and lengths; the rows and the table's
 // entry; the page's scale; its codes, when the scale grows).
 template <bool F16>
 __global__ void __launch_bounds__(256) k_cache_write(const CacheArgs c, const int* __restrict__ offsets,
@@ -190,7 +190,8 @@ __global__ void __launch_bounds__(256) k_cache_write(const CacheArgs c, const in
 }
 
 // ---- read: the same blocks; code * scale in 16 bits (exact in bf16; rounded once where fp16's range
-// ends).  DENSE: every position, to row s * table_ld * 64 + position.  Bound by the bytes: 1 in, 2 out.
+// ends).  DENSE: every position, to row s * table_ld * 64 + position.  Bound by the bytes, 1 in, 2 out
+// (7417 rows of 8 heads: 7.1 us, 6.4 TB/s).
 template <bool F16, bool DENSE>
 __global__ void __launch_bounds__(256) k_cache_read(const CacheArgs c, const int* __restrict__ offsets,
                                                     long long rows, uint16_t* __restrict__ k, long long ld_k,
@@ -267,7 +268,10 @@ __global__ void __launch_bounds__(256) k_cache_read(const CacheArgs c, const int
 // the launch's tag, a number that no other launch of the process has, so whatever the workspace held before
 // is not taken for one.
 //
-// Bound by the codes' bytes (a code takes part in 4 g c operations) as long as the instructions keep up.
+// Bound by the codes' bytes (a code takes part in 4 g c operations) as long as the instructions keep up: 64
+// tokens over 500 to 8192 positions each, 335 MB, take 66.8 us (5.0 TB/s; 6.2 from the first copy to the last), one
+// over 130001, 266 MB, 54 us.  One over 1001 takes 9.7 us, all latency: launch 1.4, lengths and cut 1.8, the
+// first span 2.7, the join over memory 3.
 // A byte permute, a logical operation and a paired fp16 one each take a scheduler two clocks a warp, an
 // MMA eight, so what turns codes into operands is what counts:
 //   * codes are the 16-row operand and the queries the 8 columns: S^T = K Q^T, O^T = V^T P^T, so 8

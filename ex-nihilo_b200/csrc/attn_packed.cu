@@ -35,6 +35,12 @@
 // The sums and maxima are fp32; P is rounded to the inputs' 16-bit type (the
 // tensor core's operand), o once at the end.
 //
+// Bound by the chain S, maximum, exponentials, P, PV of a unit, 0.98 us for both tiles: at 8192 causal rows of
+// 32 heads over 8 (452 us, 1216 TFLOP/s) the tensor pipe is busy 56 % of the time, the exponentials' 57 %, the
+// schedulers 42 %.  A fourth of the exponentials as polynomials (491 us), no turns between the two tiles (476 us) and
+// two warps a row (520 us) were slower.  A short item costs about 5 us besides its units, most of which
+// overlaps with the next one's loads; a launch of one prompt of 27 rows takes 6.5 us.
+//
 // A hidden key's P is 0, and 0 times a V that is infinite or NaN would still
 // be NaN in the tensor core: such V rows can belong to the next sequence or to
 // a later token.  So an output row that comes out not finite is looked at
