@@ -295,6 +295,25 @@ def test_packed_captured_with_shared_items(att):
             check_packed(out, q, k, v, nq, heads, kv_heads, "bf16", nk=nk)
 
 
+def test_packed_past_32_bits(att):
+    """Thousands of sequences whose rows reach past 2^31 elements: those around the border and the last."""
+    heads, kv_heads, each, nseq = 32, 8, 61, 8700
+    n = each * nseq
+    assert n * heads * D > 2 ** 31
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.empty(n, heads * D, dtype=torch.bfloat16, device="cuda")
+    q[-40 * each:] = rows(40 * each, heads, 1, "bf16")
+    border = 2 ** 31 // (heads * D) // each * each
+    q[:border - each].fill_(0.5)
+    q[border - each:border + 2 * each] = rows(3 * each, heads, 2, "bf16")
+    q[border + 2 * each:-40 * each].fill_(0.5)
+    k = torch.randn(n, kv_heads * D, generator=g, device="cuda", dtype=torch.bfloat16).clamp_(-1.4, 1.4)
+    v = torch.randn(n, kv_heads * D, generator=g, device="cuda", dtype=torch.bfloat16)
+    out = run_packed(att, q, k, v, [each] * nseq, heads, kv_heads, "bf16")
+    for a in (0, border - each, border, border + each, n - 3 * each, n - each):
+        check(out[a:a + each], reference(q[a:a + each], k[a:a + each], v[a:a + each], heads, kv_heads), "bf16")
+
+
 # --------------------------------------------------------------------------- the cache
 
 
@@ -683,6 +702,31 @@ def test_rows_before_the_first_position_are_zero(att, extra):
     out = c.attend(att, counts, q, heads, "bf16")
     c.check_attend(out, counts, q, heads, "bf16")
     assert (out[:extra] == 0).all() and (out[100 + extra:102 + extra] == 0).all()
+
+
+@pytest.mark.parametrize("tokens", [1, 5, 150])
+def test_cache_past_32_bits(att, tokens):
+    """A pool of more than 4 GB of codes whose last pages are the sequences': written, read and attended."""
+    heads, kv_heads = 16, 8
+    c = Cache(2, 5, kv_heads)
+    pages = 2 ** 32 // (kv_heads * 64 * D) + 11
+    codes = {x: torch.empty(pages, kv_heads, 64, D, dtype=torch.int8, device="cuda") for x in "kv"}
+    scales = {x: torch.full((pages, kv_heads), 2.0 ** 40, device="cuda") for x in "kv"}
+    c.codes, c.scales = codes, scales
+    c.c.k, c.c.v = codes["k"].data_ptr(), codes["v"].data_ptr()
+    c.c.k_scale, c.c.v_scale, c.c.pages = scales["k"].data_ptr(), scales["v"].data_ptr(), pages
+    c.table.copy_((pages - 1 - torch.arange(10, device="cuda")).int().reshape(2, 5))
+    lens = [161, 99]
+    k, v = rows(260, kv_heads, 1, "bf16"), rows(260, kv_heads, 2, "bf16")
+    c.write(att, lens, k, v, "bf16")
+    new = [tokens, min(tokens, 2)]
+    k, v, q = rows(sum(new), kv_heads, 3, "bf16"), rows(sum(new), kv_heads, 4, "bf16"), rows(sum(new), heads, 5, "bf16")
+    c.write(att, new, k, v, "bf16")
+    total = [a + b for a, b in zip(lens, new)]
+    got_k, got_v = c.read(att, total, "bf16")
+    assert torch.equal(got_k.double(), c.expect("k", total).flatten(1))
+    assert torch.equal(got_v.double(), c.expect("v", total).flatten(1))
+    c.check_attend(c.attend(att, new, q, heads, "bf16"), new, q, heads, "bf16")
 
 
 # --------------------------------------------------------------------------- refusals
