@@ -761,6 +761,19 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
 
   // ---- the computing warps
   auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); };
+  // the same, and whether all are OK: no warp leaves after a wait that ran out while another waits for it here
+  auto together = [](bool ok) -> bool {
+    int all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.s32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, 1, %2, p;\n\t"
+        "selp.s32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"(static_cast<int>(ok)), "n"(THREADS)
+        : "memory");
+    return all != 0;
+  };
   const uint32_t ring32 = smem_u32(smem + warp * SLOTS * SPAN_BYTES);
   uint64_t* const full = sh.full[warp];
   uint64_t* const empty = sh.empty[warp];
@@ -779,7 +792,7 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
 
   for (int k = 0;; ++k) {
     const int b = k & 1;
-    ok = ok && mbar_wait_uniform(&sh.seg_full[b], (k >> 1) & 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+    ok = together(mbar_wait_uniform(&sh.seg_full[b], (k >> 1) & 1, abort_flag, status, STATUS_TIMEOUT_ATTN));
     if (!ok) break;
     const int n = sh.seg[b].n, nh = sh.seg[b].nh, nrows = sh.seg[b].tok * nh, pos0 = sh.seg[b].pos0;
     if (n == 0) break;
@@ -1000,7 +1013,6 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
       }
       step();
     }
-    if (!ok) break;
     turn -= n;
 
     // ---- join the warps: o = sum_w 2^(m_w - M) o_w, l likewise, in a fixed order
@@ -1024,7 +1036,8 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
       }
     const Seg seg = sh.seg[b];
     const int part_len = sh.part_len, lead = sh.lead;
-    barrier();
+    ok = together(ok);
+    if (!ok) break;
     if (lane == 0) mbar_arrive(&sh.seg_empty[b]);
     const bool whole = n == seg.spans;
     // a row's four values at 4 (x & 31), normalised and stored

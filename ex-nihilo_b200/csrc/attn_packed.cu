@@ -273,11 +273,11 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
 
   // The waits for the next item are the only ones that do not look at the abort flag, so every role goes through
   // the same items, with the work left out once a wait has run out, and the tiles' warps stay in step.  The
-  // producer, whose own waits are bounded, ends the list.
+  // producer, whose own waits are shorter, ends the list.
   volatile int no_abort = 0;
-  auto wait_item = [&](uint64_t* bar, uint32_t parity) {  // one thread
+  auto wait_item = [&](uint64_t* bar, uint32_t parity, int limits = 16) {  // one thread
     volatile int none = 0;
-    return mbar_wait(bar, parity, &none, status, STATUS_TIMEOUT_ATTN, 16 * EXN_WAIT_NS);
+    return mbar_wait(bar, parity, &none, status, STATUS_TIMEOUT_ATTN, limits * EXN_WAIT_NS);
   };
 
   bool joined = false;
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       x.kvh = -1;
       while (!ended && ok) {
         if (!asked) ask();
-        if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->claim_full, claims & 1) : true, 0)) {
+        if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->claim_full, claims & 1, 1) : true, 0)) {
           ok = false;
           return;
         }
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     for (uint32_t k = 0;; ++k) {
       const int ib = k & 1;
       if (*abort_flag) ok = false;
-      if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->item_empty[ib], ((k >> 1) & 1) ^ 1) : true, 0)) ok = false;
+      if (!__shfl_sync(0xffffffffu, lane == 0 ? wait_item(&bars->item_empty[ib], ((k >> 1) & 1) ^ 1, 8) : true, 0)) ok = false;
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) cur.kvh = -1;
       if (lane == 0) {
