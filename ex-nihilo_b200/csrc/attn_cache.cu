@@ -87,25 +87,25 @@ __device__ __forceinline__ void find_page(const int* offsets, const int* lens, i
   __syncthreads();
 }
 
-// ---- write: one block = one page touched by the call's rows, one key/value head; threads 0..127 take
-// K, 128..255 V, 16 threads a row of 128 values.  Long prompts are bound by the bytes, 2 in and 1 out a
-// value (6360 rows of 8 heads: 8.3 us, 4.7 TB/s); single tokens (64: 5.0 us) by the chain of dependent loads (offsets and lengths; the rows and the table's
-// entry; the page's scale; its codes, when the scale grows).
+// ---- write: one block = one page touched by the call's rows, one key/value head, K or V; 16 threads a row of
+// 128 values.  Long prompts are bound by the bytes, 2 in and 1 out a value (6360 rows of 8 heads: 7.9 us, 5.0
+// TB/s); single tokens (64: 4.5 us) by the chain of dependent loads (offsets and lengths; the rows and the
+// table's entry; the page's scale; its codes, when the scale grows).
 template <bool F16>
-__global__ void __launch_bounds__(256) k_cache_write(const CacheArgs c, const int* __restrict__ offsets,
+__global__ void __launch_bounds__(128) k_cache_write(const CacheArgs c, const int* __restrict__ offsets,
                                                      long long rows, const uint16_t* __restrict__ k, long long ld_k,
                                                      const uint16_t* __restrict__ v, long long ld_v, int* status) {
   __shared__ PageRows at;
-  __shared__ uint32_t red[8];
-  const int slot = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads;
+  __shared__ uint32_t red[4];
+  const int slot = blockIdx.x / (2 * c.kv_heads), h = blockIdx.x % (2 * c.kv_heads) >> 1;
   griddep_wait();
   griddep_launch();
   find_page(offsets, c.lens, c.nseq, rows, slot, &at, status);
   if (at.s < 0) return;
   const int page = at.page_i < c.table_ld ? c.table[static_cast<long long>(at.s) * c.table_ld + at.page_i] : -1;
   const int lo = at.lo, hi = at.hi;
-  const bool is_v = threadIdx.x >= 128;
-  const int tid = threadIdx.x & 127, sub = tid & 15, r0 = tid >> 4;  // 8 values at 8 sub of rows r0, r0 + 8, ..
+  const bool is_v = blockIdx.x & 1;
+  const int sub = threadIdx.x & 15, r0 = threadIdx.x >> 4;  // 8 values at 8 sub of rows r0, r0 + 8, ..
   const long long ld = is_v ? ld_v : ld_k;
   const uint16_t* src = (is_v ? v : k) + at.row0 * ld + h * 128 + sub * 8;
 
@@ -133,8 +133,7 @@ __global__ void __launch_bounds__(256) k_cache_write(const CacheArgs c, const in
   for (int o = 16; o > 0; o >>= 1) mag = __vmaxu2(mag, __shfl_xor_sync(0xffffffffu, mag, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mag;
   __syncthreads();
-  const int w0 = is_v ? 4 : 0;
-  mag = __vmaxu2(__vmaxu2(red[w0], red[w0 + 1]), __vmaxu2(red[w0 + 2], red[w0 + 3]));
+  mag = __vmaxu2(__vmaxu2(red[0], red[1]), __vmaxu2(red[2], red[3]));
   const float amax = unpack16<F16>(max(mag & 0xffffu, mag >> 16)).x;
   const bool poisoned = !(amax < INFINITY) || before != before;  // infinite or NaN
   const float mine = pow2(scale_exponent(poisoned ? 0.f : amax));
@@ -186,18 +185,18 @@ __global__ void __launch_bounds__(256) k_cache_write(const CacheArgs c, const in
       *reinterpret_cast<uint2*>(dst + r * 128) = make_uint2(u[0], u[1]);
     }
   }
-  if (tid == 0) *scale = poisoned ? __uint_as_float(0x7fffffffu) : now;
+  if (threadIdx.x == 0) *scale = poisoned ? __uint_as_float(0x7fffffffu) : now;
 }
 
 // ---- read: the same blocks; code * scale in 16 bits (exact in bf16; rounded once where fp16's range
 // ends).  DENSE: every position, to row s * table_ld * 64 + position.  Bound by the bytes, 1 in, 2 out
-// (7417 rows of 8 heads: 7.1 us, 6.4 TB/s).
+// (7417 rows of 8 heads: 6.9 us, 6.6 TB/s).
 template <bool F16, bool DENSE>
-__global__ void __launch_bounds__(256) k_cache_read(const CacheArgs c, const int* __restrict__ offsets,
+__global__ void __launch_bounds__(128) k_cache_read(const CacheArgs c, const int* __restrict__ offsets,
                                                     long long rows, uint16_t* __restrict__ k, long long ld_k,
                                                     uint16_t* __restrict__ v, long long ld_v, int* status) {
   __shared__ PageRows found;
-  const int slot = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads;
+  const int slot = blockIdx.x / (2 * c.kv_heads), h = blockIdx.x % (2 * c.kv_heads) >> 1;
   griddep_wait();
   griddep_launch();
   PageRows at;
@@ -223,8 +222,8 @@ __global__ void __launch_bounds__(256) k_cache_read(const CacheArgs c, const int
     if (threadIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
     return;
   }
-  const bool is_v = threadIdx.x >= 128;
-  const int tid = threadIdx.x & 127, sub = tid & 15, r0 = tid >> 4;
+  const bool is_v = blockIdx.x & 1;
+  const int sub = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   const long long head = static_cast<long long>(page) * c.kv_heads + h;
   const int8_t* src = (is_v ? c.v : c.k) + head * PAGE_BYTES + sub * 8;
   const float scale = (is_v ? c.v_scale : c.k_scale)[head];
@@ -1178,28 +1177,28 @@ unsigned long long launch_tag() {
 
 int cache_write_launch(const CacheArgs& c, int f16, const int* offsets, long long rows, const void* k, long long ld_k,
                        const void* v, long long ld_v, int* d_status, cudaStream_t st) {
-  const long long blocks = (rows / kPage + 2ll * c.nseq) * c.kv_heads;
+  const long long blocks = (rows / kPage + 2ll * c.nseq) * c.kv_heads * 2;
   if (blocks > 0x7fffffffll) return -1;
   return static_cast<int>(launch_pdl(f16 ? k_cache_write<true> : k_cache_write<false>,
-                                     dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, c, offsets, rows,
+                                     dim3(static_cast<unsigned>(blocks)), dim3(128), 0, st, c, offsets, rows,
                                      static_cast<const uint16_t*>(k), ld_k, static_cast<const uint16_t*>(v), ld_v, d_status));
 }
 
 int cache_read_launch(const CacheArgs& c, int f16, const int* offsets, long long rows, void* k, long long ld_k,
                       void* v, long long ld_v, int* d_status, cudaStream_t st) {
-  const long long blocks = (rows / kPage + 2ll * c.nseq) * c.kv_heads;
+  const long long blocks = (rows / kPage + 2ll * c.nseq) * c.kv_heads * 2;
   if (blocks > 0x7fffffffll) return -1;
   return static_cast<int>(launch_pdl(f16 ? k_cache_read<true, false> : k_cache_read<false, false>,
-                                     dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, c, offsets, rows,
+                                     dim3(static_cast<unsigned>(blocks)), dim3(128), 0, st, c, offsets, rows,
                                      static_cast<uint16_t*>(k), ld_k, static_cast<uint16_t*>(v), ld_v, d_status));
 }
 
 static int dense_launch(const CacheArgs& c, int f16, void* k, void* v, int* d_status, cudaStream_t st) {
-  const long long blocks = static_cast<long long>(c.nseq) * c.table_ld * c.kv_heads;
+  const long long blocks = static_cast<long long>(c.nseq) * c.table_ld * c.kv_heads * 2;
   if (blocks > 0x7fffffffll) return -1;
   const long long ld = static_cast<long long>(c.kv_heads) * 128;
   return static_cast<int>(launch_pdl(f16 ? k_cache_read<true, true> : k_cache_read<false, true>,
-                                     dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, c, static_cast<const int*>(nullptr),
+                                     dim3(static_cast<unsigned>(blocks)), dim3(128), 0, st, c, static_cast<const int*>(nullptr),
                                      0ll, static_cast<uint16_t*>(k), ld, static_cast<uint16_t*>(v), ld, d_status));
 }
 
