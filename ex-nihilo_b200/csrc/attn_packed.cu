@@ -124,12 +124,18 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const uint32_t* v) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
                : "memory");
+  return v;
 }
-__device__ __forceinline__ void st_cluster_f2(uint32_t addr, float a, float b) {
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1,%2};" ::"r"(addr), "f"(a), "f"(b) : "memory");
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
 }
 
 static_assert(sizeof(Bars) <= 512, "the barriers' room");
@@ -671,17 +677,14 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       }
       units += n;
       if (SPLIT && it.share) {
-        // ---- the join of a cluster's parts.  Every CTA owns PER rows: all send their share of O (fp32) and (m, l)
-        // there, over Q's and the ring's memory (16 bytes i of the owner's row j at i ^ (j % 32)), and the owner joins
-        // them, a warp a row.
+        // ---- the join of a cluster's parts.  Every CTA leaves its O (fp32) and (m, l) over Q's and the ring's memory
+        // (16 bytes i of row j at i ^ (j % 32)); then each takes a share of the rows, a warp 32 / parts of them.
         if (n > 0) ok = ok && mbar_wait_uniform(&bars->o_full[x], 0, abort_flag, status, STATUS_TIMEOUT_ATTN);
         tc_fence_after();
-        cluster_sync();  // every CTA's MMAs are done
-        const int per = 2 * TILE / parts;
+        asm volatile("bar.sync 9, 256;" ::: "memory");  // the softmax warps': both tiles' MMAs are done
         float2* const ml = reinterpret_cast<float2*>(smem + OFF_SLOT + 2 * TILE_BYTES);
         {
-          const int row = x * TILE + r, j = row % per, owner = row / per;
-          const uint32_t dst = mapa_shared(smem + (part * per + j) * 512, owner);
+          float4* const mine = reinterpret_cast<float4*>(smem + (x * TILE + r) * 512);
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t rr[32];
@@ -692,43 +695,77 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
               for (int i = 0; i < 32; ++i) rr[i] = 0u;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) st_cluster_v4(dst + (((c * 8 + i) ^ (j & 31)) << 4), rr + 4 * i);
+            for (int i = 0; i < 8; ++i)
+              mine[(c * 8 + i) ^ lane] = make_float4(__uint_as_float(rr[4 * i]), __uint_as_float(rr[4 * i + 1]),
+                                                     __uint_as_float(rr[4 * i + 2]), __uint_as_float(rr[4 * i + 3]));
           }
-          st_cluster_f2(mapa_shared(ml + part * per + j, owner), m, lsum);
+          ml[x * TILE + r] = make_float2(m, lsum);
         }
         cluster_sync();
+        const int shift = 31 - __clz(parts), row0 = (part * 8 + warp - 3) * (32 >> shift);  // the warp's first row
+        // a lane a (row, part): its weight 2^(m_c - M) / l, and of the first lanes each a row: where it goes
+        float weight;
+        {
+          const float2 y = ld_cluster_f2(mapa_shared(ml + row0 + (lane >> shift), lane & (parts - 1)));
+          float mx = y.x;
+          for (int o = 1; o < parts; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+          weight = fast_exp2(y.x - (mx == -INFINITY ? 0.f : mx));
+          float l = weight * y.y;
+          for (int o = 1; o < parts; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+          weight = l == 0.f ? 0.f : weight / l;
+        }
+        const int row = row0 + lane, y = row / TILE, rj = row - y * TILE, tj = rj / g, token = it.t0 + y * tpt + tj;
+        const bool valid = lane < (32 >> shift) && y < tiles && tj < tpt && token < nq;
+        const int head = kvh * g + rj - tj * g;
+        const unsigned rows_mask = __ballot_sync(0xffffffffu, valid);
 #pragma unroll 1
-        for (int j = warp - 3; j < per; j += 8) {
-          const int row = part * per + j, y = row / TILE, rj = row - y * TILE, tj = rj / g, token = it.t0 + y * tpt + tj;
-          if (y >= tiles || tj >= tpt || token >= nq) continue;
-          float mx = -INFINITY, l = 0.f;
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int c = 0; c < parts; ++c) mx = fmaxf(mx, ml[c * per + j].x);
-          const float mu = mx == -INFINITY ? 0.f : mx;
-          for (int c = 0; c < parts; ++c) {
-            const float2 a = ml[c * per + j];
-            const float4 z = reinterpret_cast<const float4*>(smem + (c * per + j) * 512)[lane ^ (j & 31)];
-            const float w = fast_exp2(a.x - mu);
-            l += w * a.y;
-            o.x += w * z.x;
-            o.y += w * z.y;
-            o.z += w * z.z;
-            o.w += w * z.w;
+        for (int b = 0; b < 2; ++b) {  // 16 of the warp's 32 pieces at a time
+          float4 z[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = row0 + ((b * 16 + i) >> shift);
+            z[i] = ld_cluster_f4(mapa_shared(smem + j * 512 + ((lane ^ (j & 31)) << 4), i & (parts - 1)));
           }
-          const float inv = l == 0.f ? 0.f : 1.f / l;
-          o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-          const int head = kvh * g + rj - tj * g;
-          uint16_t* const dst = out + static_cast<long long>(q_start + token) * p.ld_out + head * 128;
-          reinterpret_cast<uint2*>(dst)[lane] = make_uint2(pack16<F16>(o.x, o.y), pack16<F16>(o.z, o.w));
-          if (__any_sync(0xffffffffu, !(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w)))) {
-            const long long seen = min(nq, it.t0 + (y + 1) * tpt) + delta;  // by the tile's last row
-            const long long end = min((seen + UNIT - 1) / UNIT * UNIT, p.kv_rows - k_start), k0 = k_start;
-            mend_row<F16>(static_cast<const uint16_t*>(p.q) + static_cast<long long>(q_start + token) * p.ld_q + head * 128,
-                          static_cast<const uint16_t*>(p.k) + k0 * p.ld_k + kvh * 128, p.ld_k,
-                          static_cast<const uint16_t*>(p.v) + k0 * p.ld_v + kvh * 128, p.ld_v, token + delta,
-                          static_cast<int>(end) - 1, p.scale_log2, dst);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float w = __shfl_sync(0xffffffffu, weight, b * 16 + i);
+            z[i] = make_float4(w * z[i].x, w * z[i].y, w * z[i].z, w * z[i].w);
+          }
+          // the sums over 2, 4 or 8 parts move to the front
+#pragma unroll
+          for (int s2 = 1; s2 < 8; s2 *= 2)
+            if (s2 < parts)
+#pragma unroll
+              for (int i = 0; i < 8 / s2; ++i)
+                z[i] = make_float4(z[2 * i].x + z[2 * i + 1].x, z[2 * i].y + z[2 * i + 1].y, z[2 * i].z + z[2 * i + 1].z,
+                                   z[2 * i].w + z[2 * i + 1].w);
+          const int k0 = (b * 16) >> shift;
+          unsigned bad = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int k = k0 + i, to = __shfl_sync(0xffffffffu, token, k), h = __shfl_sync(0xffffffffu, head, k);
+            if (i < (16 >> shift) && ((rows_mask >> k) & 1)) {
+              const float4 o = z[i];
+              reinterpret_cast<uint2*>(out + static_cast<long long>(q_start + to) * p.ld_out + h * 128)[lane] =
+                  make_uint2(pack16<F16>(o.x, o.y), pack16<F16>(o.z, o.w));
+              if (!(isfinite(o.x) && isfinite(o.y) && isfinite(o.z) && isfinite(o.w))) bad |= 1u << k;
+            }
+          }
+          bad = __reduce_or_sync(0xffffffffu, bad);
+          while (bad) {
+            const int k = __ffs(bad) - 1, to = __shfl_sync(0xffffffffu, token, k), h = __shfl_sync(0xffffffffu, head, k);
+            bad &= bad - 1;
+            const long long seen = min(nq, it.t0 + ((row0 + k) / TILE + 1) * tpt) + delta;  // by the tile's last row
+            const long long end = min((seen + UNIT - 1) / UNIT * UNIT, p.kv_rows - k_start), kr = k_start;
+            mend_row<F16>(static_cast<const uint16_t*>(p.q) + static_cast<long long>(q_start + to) * p.ld_q + h * 128,
+                          static_cast<const uint16_t*>(p.k) + kr * p.ld_k + kvh * 128, p.ld_k,
+                          static_cast<const uint16_t*>(p.v) + kr * p.ld_v + kvh * 128, p.ld_v, to + delta,
+                          static_cast<int>(end) - 1, p.scale_log2,
+                          out + static_cast<long long>(q_start + to) * p.ld_out + h * 128);
+            __syncwarp();
           }
         }
+        cluster_sync();  // no CTA leaves while another reads its parts
         joined = true;
         break;  // a cluster has one item
       }
