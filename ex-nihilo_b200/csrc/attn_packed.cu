@@ -64,7 +64,7 @@ constexpr int TILE_BYTES = 2 * HALF;  // 32 KB
 constexpr int SLOTS = 4;              // K_0 V_0 K_1 V_1 ... stream through 4 slots
 constexpr int OFF_QA = 0, OFF_QB = TILE_BYTES, OFF_SLOT = 2 * TILE_BYTES, OFF_BAR = (2 + SLOTS) * TILE_BYTES;
 constexpr int PK_SMEM = OFF_BAR + 512 + 1024;
-constexpr int MIN_SHARED = 1024;           // keys of an item that is worth a cluster
+constexpr int MIN_SHARED = 768;            // keys of an item that is worth a cluster
 constexpr float RESCALE_THRESHOLD = 8.0f;  // log2 units
 
 // kind::f16 instruction descriptor for 16-bit operands of one type (bf16 or fp16) and fp32 sums
@@ -897,17 +897,17 @@ int packed_launch(const PackedArgs& a, int* d_status, cudaStream_t st) {
     return -4;
   const long long nslots = (a.rows - 1) / (2 * tpt) + a.nseq, items = nslots * a.kv_heads;  // at most
   if (items > 0x7fffffffll) return -1;
-  // CTAs a cluster.  Its launch and join cost about 10 us, so it has to have keys enough to share, and all clusters
+  // CTAs a cluster.  Its launch and join cost about 5 us, so it has to have keys enough to share, and all clusters
   // run at once (74 of 2, 33 of 4, 15 of 8).  us at 1, 2, 4 and 8 CTAs an item (32 heads over 8, bf16):
-  //   64 rows (8 items)    over  1024 keys:  22   25   20   21    over 16384 keys: 249  138   76   49
-  //   192 rows (32 items)  over  1024 keys:  23   26   21   38    over  8192 keys: 128   78   48   65
-  //   512 rows (72 items)  over  1024 keys:  23   26   42   87    over  8192 keys: 130   80   96  153
+  //   64 rows (8 items)    over 512 keys:  15 15 14 16    over  768: 18 17 16 16    over 16384: 247 134  73  46
+  //   192 rows (24 items)  over 512 keys:  15 15 15       over  768: 19 18 17       over  8192: 128  73  45
+  //   512 rows (64 items)  over 512 keys:  15 16          over 1024: 23 20          over  8192: 128  75
   // Up to twice the clusters of 2, some items are shared; with one sequence, whose items are alike, that gains
-  // nothing (1024 rows over 1100 keys: 24 us alone, 30 so), with several it does when their keys differ (300, 77,
-  // 512 and 9 rows over 4100, 900, 513 and 5 keys, 28 heads over 4: 69 us alone, 51 so).
+  // nothing (1024 rows over 1100 keys: 24 us either way), with several it does when their keys differ (300, 77,
+  // 512 and 9 rows over 4100, 900, 513 and 5 keys, 28 heads over 4: 68 us alone, 44 so).
   const long long keys = a.kv_rows / a.nseq;
   const int parts = keys < MIN_SHARED ? 1 : items <= a.fit[2] ? 8 : items <= a.fit[1] ? 4
-                    : keys >= 2048 && items <= a.fit[0] ? 2 : a.nseq > 1 && a.nseq <= 32 && items <= 2 * a.fit[0] ? 2 : 1;
+                    : items <= (a.nseq > 1 && a.nseq <= 32 ? 2 : 1) * a.fit[0] ? 2 : 1;
   const int fit = parts > 1 ? a.fit[parts == 8 ? 2 : parts == 4 ? 1 : 0] : 0;
   const PackedLaunch l(static_cast<unsigned>(parts > 1 && items > fit ? fit : items), parts, st);
   auto* const kernel = parts > 1 ? (a.f16 ? k_packed<true, true> : k_packed<false, true>)
