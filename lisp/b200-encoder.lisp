@@ -52,6 +52,41 @@
   (positions sb-sys:system-area-pointer)
   (states sb-sys:system-area-pointer))
 
+(sb-alien:define-alien-routine ("exn_enc_states_packed" %enc-states-packed) sb-alien:int
+  (e sb-sys:system-area-pointer)
+  (ids sb-sys:system-area-pointer)
+  (nseq sb-alien:int)
+  (counts sb-sys:system-area-pointer)
+  (positions sb-sys:system-area-pointer)
+  (states sb-sys:system-area-pointer))
+
+(sb-alien:define-alien-routine ("exn_enc_cache_open" %enc-cache-open) sb-alien:int
+  (e sb-sys:system-area-pointer)
+  (nseq sb-alien:int)
+  (max-tokens sb-alien:int)
+  (out (* sb-sys:system-area-pointer)))
+
+(sb-alien:define-alien-routine ("exn_enc_cache_close" %enc-cache-close) sb-alien:void
+  (c sb-sys:system-area-pointer))
+
+(sb-alien:define-alien-routine ("exn_enc_cache_trim" %enc-cache-trim) sb-alien:int
+  (e sb-sys:system-area-pointer)
+  (c sb-sys:system-area-pointer)
+  (seq sb-alien:int)
+  (tokens sb-alien:int))
+
+(sb-alien:define-alien-routine ("exn_enc_cache_length" %enc-cache-length) sb-alien:int
+  (c sb-sys:system-area-pointer)
+  (seq sb-alien:int))
+
+(sb-alien:define-alien-routine ("exn_enc_extend" %enc-extend) sb-alien:int
+  (e sb-sys:system-area-pointer)
+  (c sb-sys:system-area-pointer)
+  (ids sb-sys:system-area-pointer)
+  (counts sb-sys:system-area-pointer)
+  (positions sb-sys:system-area-pointer)
+  (states sb-sys:system-area-pointer))
+
 (sb-alien:define-alien-routine ("exn_enc_release" %enc-release) sb-alien:int
   (e sb-sys:system-area-pointer))
 
@@ -104,6 +139,51 @@
                                     (if pos (sb-sys:vector-sap pos) (sb-sys:int-sap 0))
                                     (sb-sys:vector-sap all))))
     all))
+
+;;; --- several prompts at once, and prompts that grow (no counterpart in the reference) ----
+
+(defun call-on-prompts (model prompts function)
+  "FUNCTION on the pointers to the ids of PROMPTS one after another, their counts and the states, which
+   it fills: each prompt's states, as encoder-states returns them."
+  (let* ((d (genc-width model))
+         (counts (map '(vector (signed-byte 32)) #'length prompts))
+         (ids (coerce (loop for p in prompts append (coerce p 'list)) '(vector (signed-byte 32))))
+         (all (make-array (* (length ids) d) :element-type 'single-float)))
+    (sb-sys:with-pinned-objects (counts ids all)
+      (enc-check model (funcall function (sb-sys:vector-sap ids) (sb-sys:vector-sap counts)
+                                (sb-sys:vector-sap all))))
+    (loop for n across counts
+          for end = (* n d) then (+ end (* n d))
+          collect (subseq all (- end (* n d)) end))))
+
+(defun encoder-states-packed (model prompts)
+  "encoder-states of each of PROMPTS, a list of lists of ids, in one pass over the weights."
+  (call-on-prompts model prompts
+                   (lambda (ids counts states)
+                     (%enc-states-packed (genc-handle model) ids (length prompts) counts
+                                         (sb-sys:int-sap 0) states))))
+
+(defun open-prompt-cache (model count max-tokens)
+  "Room for the keys and values of COUNT prompts of up to MAX-TOKENS tokens on MODEL's GPU."
+  (sb-alien:with-alien ((c sb-sys:system-area-pointer))
+    (enc-check model (%enc-cache-open (genc-handle model) count max-tokens (sb-alien:addr c)))
+    c))
+
+(defun close-prompt-cache (cache)
+  (%enc-cache-close cache))
+
+(defun extend-prompts (model cache tokens)
+  "More tokens of every prompt of CACHE, a list of lists of ids (NIL: none): their states."
+  (call-on-prompts model tokens
+                   (lambda (ids counts states)
+                     (%enc-extend (genc-handle model) cache ids counts (sb-sys:int-sap 0) states))))
+
+(defun trim-prompt (model cache seq tokens)
+  "Keep the first TOKENS tokens of prompt SEQ."
+  (enc-check model (%enc-cache-trim (genc-handle model) cache seq tokens)))
+
+(defun prompt-length (cache seq)
+  (%enc-cache-length cache seq))
 
 (defun encoder-release (model)
   "The encoder's scratch freed (the weights stay)."
