@@ -441,19 +441,20 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
       __syncwarp();
       if (cur.kvh < 0) break;
       // a tile of Q: the box (64 dims, g heads, tpt tokens), rows token-major; rows of the tile past g tpt stay
-      // as they are and are never stored
-      if (cur.nloads > 0)
-        for (int x = 0; x < cur.tiles; ++x) {
-          ok = ok && mbar_wait_warp(&bars->q_empty[x], (q_count[x] & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
-          if (!ok) break;
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&bars->q_full[x], 2 * g * tpt * 128);
-            for (int hf = 0; hf < 2; ++hf)
-              tma_load_3d(smem + (x ? OFF_QB : OFF_QA) + hf * HALF, &tmQ, &bars->q_full[x], hf * 64, cur.kvh * g,
-                          cur.q_start + cur.t0 + x * tpt);
-          }
-          ++q_count[x];
+      // as they are and are never stored.  Only for a tile that has units here: its product's end is what the
+      // softmax warps wait for before they write over Q's memory, so no copy may be left that nothing waits for.
+      for (int x = 0; x < cur.tiles; ++x) {
+        if (cur.nu[x] == 0) continue;
+        ok = ok && mbar_wait_warp(&bars->q_empty[x], (q_count[x] & 1) ^ 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->q_full[x], 2 * g * tpt * 128);
+          for (int hf = 0; hf < 2; ++hf)
+            tma_load_3d(smem + (x ? OFF_QB : OFF_QA) + hf * HALF, &tmQ, &bars->q_full[x], hf * 64, cur.kvh * g,
+                        cur.q_start + cur.t0 + x * tpt);
         }
+        ++q_count[x];
+      }
       Item next;
       for (int t = 0; t < 2 * cur.nloads; ++t) {
         if (t >= 2 * cur.nloads - 8 && !asked && !ended) ask();
@@ -515,13 +516,12 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         const int ib = k & 1;
         if (!wait_item(&bars->item_full[ib], (k >> 1) & 1)) break;
         const int n = bars->item[ib].nu[x], nloads = bars->item[ib].nloads;
-        const bool has_q = nloads > 0 && x < bars->item[ib].tiles, last = bars->item[ib].kvh < 0;
+        const bool last = bars->item[ib].kvh < 0;
         mbar_arrive(&bars->item_empty[ib]);
         if (last) break;
-        if (has_q) {
+        if (n > 0) {
           ok = ok && mbar_wait(&bars->q_full[x], q_count & 1, abort_flag, status, STATUS_TIMEOUT_ATTN);
           ++q_count;
-          if (ok && n == 0) umma_commit(&bars->q_empty[x]);
         }
         if (ok && n > 0 && (ok = wait_load(0))) {
           tc_fence_after();
