@@ -61,29 +61,38 @@ struct PageRows {
   int lo, hi;       // the page's rows of this call: lo .. hi - 1
   long long row0;   // the row of the page's position 0 (below 0 where the call starts inside the page)
 };
-// all threads; FOUND is shared by the block
+// All threads; FOUND is shared by the block.  From the first sequence whose offsets decrease on there are none: a
+// later one could own rows and slots of an earlier one, so that two threads would fill FOUND.  Before it the
+// sequences' slots are disjoint.
 __device__ __forceinline__ void find_page(const int* offsets, const int* lens, int nseq, long long rows, int slot,
                                           PageRows* found, int* status) {
-  if (threadIdx.x == 0) found->s = -1;
+  __shared__ int decrease;
+  if (threadIdx.x == 0) {
+    found->s = -1;
+    decrease = nseq;
+  }
   __syncthreads();
+  PageRows mine = {-1, 0, 0, 0, 0};
   for (int s = threadIdx.x; s < nseq; s += blockDim.x) {
     const int a = offsets[s], b = offsets[s + 1], len = lens[s];
+    if (b < a) atomicMin(&decrease, s);
     if (a < 0 || b < a || b > rows || len < b - a) {
       if (blockIdx.x == 0) atomicOr(status, STATUS_BAD_ARG);
       continue;
     }
-    if (b == a) continue;
+    if (b == a || mine.s >= 0) continue;
     const int pos0 = len - (b - a), p0 = pos0 / kPage, p1 = (len - 1) / kPage;
     const long long i = slot - (a / kPage + 2ll * s);
     if (i < 0 || i > p1 - p0) continue;
-    const int page_i = p0 + static_cast<int>(i);
-    const long long base = static_cast<long long>(page_i) * kPage;
-    found->s = s;
-    found->page_i = page_i;
-    found->lo = static_cast<int>(max(pos0 - base, 0ll));
-    found->hi = static_cast<int>(min(len - base, static_cast<long long>(kPage)));
-    found->row0 = a + base - pos0;
+    mine.s = s;
+    mine.page_i = p0 + static_cast<int>(i);
+    const long long base = static_cast<long long>(mine.page_i) * kPage;
+    mine.lo = static_cast<int>(max(pos0 - base, 0ll));
+    mine.hi = static_cast<int>(min(len - base, static_cast<long long>(kPage)));
+    mine.row0 = a + base - pos0;
   }
+  __syncthreads();
+  if (mine.s >= 0 && mine.s < decrease) *found = mine;
   __syncthreads();
 }
 
@@ -463,17 +472,27 @@ __device__ __forceinline__ void attend_produce(const CUtensorMap* tmK, const CUt
   const int s_lo = min(p.c.nseq, lane * chunk), s_hi = min(p.c.nseq, s_lo + chunk);
   long long lane_work = 0;
   int items = 0, longest = 0, start = 0, end = 0, len = 0;  // start, end, len: the lane's first sequence's
-  for (int s = s_lo; s < s_hi; ++s) {
-    const int a = p.offsets[s], b = p.offsets[s + 1], l = p.c.lens[s];
-    const int n = items_of(a, b, l);
-    items += n;
-    lane_work += static_cast<long long>(n) * (spans_of(l) + SETUP);
-    if (n) longest = max(longest, spans_of(l));
-    if (s == s_lo) {
-      start = a;
-      end = b;
-      len = l;
+  int decrease = p.c.nseq;  // the sequences from the first whose offsets decrease on are left out
+  for (bool again = true; again;) {
+    const int stop = decrease;
+    lane_work = 0;
+    items = longest = 0;
+    for (int s = s_lo; s < s_hi; ++s) {
+      const int a = p.offsets[s], b = p.offsets[s + 1], l = p.c.lens[s];
+      int n = items_of(a, b, l);
+      if (b < a) decrease = min(decrease, s);
+      if (s >= decrease) n = 0;
+      items += n;
+      lane_work += static_cast<long long>(n) * (spans_of(l) + SETUP);
+      if (n) longest = max(longest, spans_of(l));
+      if (s == s_lo) {
+        start = a;
+        end = b;
+        len = l;
+      }
     }
+    decrease = __reduce_min_sync(0xffffffffu, decrease);
+    again = decrease < stop;  // once more without those behind it
   }
   bool work_here = true;
   if (__any_sync(0xffffffffu, lane_work >= (1ll << 26))) {  // 2^26 spans are 512 GB of codes

@@ -297,6 +297,8 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     struct Sequence {
       int q0, q1, k0, nk, pairs;  // rows, keys, items a head
     };
+    int decrease = p.nseq;  // the sequences from the first whose offsets decrease on are left out: their rows may be
+                            // earlier ones', and there may be more items than the host's bound
     auto read = [&](int s) {
       Sequence x;
       x.q0 = p.q_offsets[s];
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
         start = p.kv_offsets[s];
         x.nk = p.kv_offsets[s + 1] - static_cast<int>(start);
       }
-      x.pairs = x.q0 < 0 || x.q1 < x.q0 || x.q1 > p.rows ? 0 : (x.q1 - x.q0 + pair - 1) / pair;
+      x.pairs = s >= decrease || x.q0 < 0 || x.q1 < x.q0 || x.q1 > p.rows ? 0 : (x.q1 - x.q0 + pair - 1) / pair;
       if (x.pairs && (start < 0 || x.nk < 0 || start + x.nk > p.kv_rows)) {
         atomicOr(status, STATUS_BAD_ARG);
         x.pairs = 0;
@@ -323,13 +325,26 @@ __global__ void __launch_bounds__(PK_THREADS, 1)
     int pairs = 0, first = 0;  // of the lane's run: its items a head, those before it
     if (sorted) {
       if (lane < p.nseq) mine = read(lane);
+      const unsigned less = __ballot_sync(0xffffffffu, mine.q1 < mine.q0);
+      if (less && lane >= __ffs(less) - 1) mine.pairs = 0;
       pairs = mine.pairs;
       for (int j = 0; j < p.nseq; ++j) {
         const int other = __shfl_sync(0xffffffffu, mine.nk, j), n = __shfl_sync(0xffffffffu, pairs, j);
         if (other > mine.nk || (other == mine.nk && j < lane)) first += n;
       }
     } else {
-      for (int s = lane * run; s < min(p.nseq, lane * run + run); ++s) pairs += read(s).pairs;
+      int less = p.nseq;
+      for (bool again = true; again;) {
+        decrease = less;
+        pairs = 0;
+        for (int s = lane * run; s < min(p.nseq, lane * run + run); ++s) {
+          const Sequence x = read(s);
+          pairs += x.pairs;
+          if (x.q1 < x.q0) less = min(less, s);
+        }
+        less = __reduce_min_sync(0xffffffffu, less);
+        again = less < decrease;  // once more without those behind it
+      }
       first = warp_before(pairs);
     }
     auto find = [&](int index, Item& x) -> bool {  // by the whole warp; false: no such item

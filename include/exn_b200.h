@@ -294,8 +294,9 @@ int exn_enc_release(exn_enc* e);
  * The calls check what the host can see and queue kernels on STREAM (a cudaStream_t of the device; NULL
  * is CUDA's default stream): no allocation, no host wait, capturable into a CUDA graph, the current
  * device left as it was.  Lengths and tables are read when the kernels run.  What the kernels find wrong
- * there (offsets that decrease or pass ROWS, lengths shorter than a sequence's rows, a page that is not
- * the pool's) they leave out, and exn_attn_sync reports it; such a sequence's rows and pages then hold
+ * there they leave out, and exn_attn_sync reports it: a sequence whose offsets pass ROWS, whose length is
+ * shorter than its rows or one of whose pages is not the pool's, and where q's offsets (or a cache call's)
+ * decrease, that sequence and all behind it.  The rows and pages of such a sequence then hold
  * anything, other sequences' are right.  The calls keep nothing between them, so
  * calls on different streams may run at once, except on the same workspace or, where one writes, on the
  * same pages.  The same call gives the same bits again.  One thread at a time uses a handle. */
