@@ -9,13 +9,14 @@
 #include <new>
 
 #include "../../include/exn_b200.h"
+#include "../../include/exn_b200_testing.h"
 #include "exn_internal.h"
 
 using namespace exn;
 
 struct exn_attn {
   int device = 0, sms = 0, fit[3] = {0, 0, 0};
-  int* d_status = nullptr;
+  int* d_status = nullptr;  // what the kernels set, and behind it what exn_attn_sync took of it
   char err[512] = "";  // no allocation, so no exception either, on the way to the caller
 };
 
@@ -128,6 +129,17 @@ int launched(exn_attn* a, const char* fn, int r) {
   return afail(a, EXN_ECUDA, "%s: launch failed: %s", fn, cudaGetErrorString(static_cast<cudaError_t>(r)));
 }
 
+// what the kernels' status word says; a kernel that gave up comes first, since then nothing is to be trusted
+int report(exn_attn* a, int s) {
+  if (!s) return EXN_OK;
+  if (s & ~STATUS_BAD_ARG_BIT)
+    return afail(a, EXN_ETIMEOUT, "a kernel gave up waiting on its pipeline (status 0x%x)%s", s,
+                 s & STATUS_BAD_ARG_BIT ? ", and one met offsets, lengths or pages out of range" : "");
+  return afail(a, EXN_EINVAL,
+               "a kernel met offsets that decrease or pass the rows, lengths shorter than a sequence's rows, or "
+               "table entries that are not pages of the pool; it left them out");
+}
+
 }  // namespace
 
 extern "C" {
@@ -151,8 +163,8 @@ int exn_attn_open(int device, exn_attn** out) {
   const int rc = [&]() -> int {
     OnDevice on(device);
     ACK(on.rc);
-    ACK(cudaMalloc(&a->d_status, sizeof(int)));
-    ACK(cudaMemset(a->d_status, 0, sizeof(int)));
+    ACK(cudaMalloc(&a->d_status, 2 * sizeof(int)));
+    ACK(cudaMemset(a->d_status, 0, 2 * sizeof(int)));
     ACK(static_cast<cudaError_t>(packed_prepare(a->fit)));
     ACK(static_cast<cudaError_t>(cache_prepare()));
     return EXN_OK;
@@ -183,16 +195,10 @@ int exn_attn_sync(exn_attn* a, void* stream) {
   ACK(on.rc);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   int s = 0;
-  ACK(cudaMemcpyAsync(&s, a->d_status, sizeof s, cudaMemcpyDeviceToHost, st));
+  ACK(static_cast<cudaError_t>(status_take_launch(a->d_status, st)));
+  ACK(cudaMemcpyAsync(&s, a->d_status + 1, sizeof s, cudaMemcpyDeviceToHost, st));
   ACK(cudaStreamSynchronize(st));
-  if (!s) return EXN_OK;
-  ACK(cudaMemsetAsync(a->d_status, 0, sizeof(int), st));
-  ACK(cudaStreamSynchronize(st));
-  if (s & STATUS_BAD_ARG_BIT)
-    return afail(a, EXN_EINVAL,
-                 "a kernel met offsets that decrease or pass the rows, lengths shorter than a sequence's rows, or "
-                 "table entries that are not pages of the pool; it left them out");
-  return afail(a, EXN_ETIMEOUT, "a kernel gave up waiting on its pipeline (status 0x%x)", s);
+  return report(a, s);
 }
 
 int exn_attn_packed(exn_attn* a, int type, int heads, int kv_heads, int nseq, const int32_t* q_offsets,
@@ -319,6 +325,14 @@ int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int 
   p.out = out;
   p.ld_out = ld_out;
   return launched(a, fn, cache_attention(p, workspace, workspace_bytes, a->sms, a->fit, a->d_status, st));
+}
+
+// include/exn_b200_testing.h
+int exn_test_attn_report(int status, char* text, int n) {
+  exn_attn a;
+  const int rc = report(&a, status);
+  snprintf(text, n, "%s", a.err);
+  return rc;
 }
 
 }  // extern "C"

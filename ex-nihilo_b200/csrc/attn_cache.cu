@@ -1182,6 +1182,9 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
   }
 }
 
+// A bit that a kernel on another stream sets meanwhile is in what is taken or in what is left
+__global__ void k_status_take(int* status) { status[1] = atomicExch(status, 0); }
+
 // A number that no other launch of this process has and that is no likely memory content
 unsigned long long launch_tag() {
   static std::atomic<unsigned long long> next{
@@ -1219,6 +1222,11 @@ static int dense_launch(const CacheArgs& c, int f16, void* k, void* v, int* d_st
   return static_cast<int>(launch_pdl(f16 ? k_cache_read<true, true> : k_cache_read<false, true>,
                                      dim3(static_cast<unsigned>(blocks)), dim3(128), 0, st, c, static_cast<const int*>(nullptr),
                                      0ll, static_cast<uint16_t*>(k), ld, static_cast<uint16_t*>(v), ld, d_status));
+}
+
+int status_take_launch(int* status, cudaStream_t st) {
+  void* args[] = {&status};
+  return static_cast<int>(cudaLaunchKernel(reinterpret_cast<const void*>(k_status_take), dim3(1), dim3(1), args, 0, st));
 }
 
 int cache_prepare() {

@@ -189,6 +189,8 @@ int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, 
                     cudaStream_t st);
 size_t cache_attention_workspace(const CacheArgs& c, int heads, long long rows, int sms);
 int cache_prepare();
+// STATUS[1] = what STATUS[0] holds, and that 0, in one step; a cudaError_t
+int status_take_launch(int* status, cudaStream_t st);
 
 // C = A . (q d)^T with the weights as Q8_0 (gemm_q8.cu): QS int8 [N][K], DK the fp16 scales laid out
 // by k-block ([K/64][N][2], q8_scales_by_kblock_launch from GGUF's [N][K/32]).  Epilogues EPI_F32

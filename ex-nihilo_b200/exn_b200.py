@@ -136,6 +136,7 @@ def lib():
         "exn_enc_release": (ctypes.c_int, [H]),
         "exn_test_enc_last_ms": (ctypes.c_int, [H, ctypes.POINTER(ctypes.c_double)]),
         "exn_test_enc_weights_digest": (ctypes.c_int, [H, ctypes.POINTER(ctypes.c_uint64)]),
+        "exn_test_attn_report": (ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, ctypes.c_int]),
         "exn_attn_open": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(H)]),
         "exn_attn_close": (None, [H]),
         "exn_attn_last_error": (ctypes.c_char_p, [H]),

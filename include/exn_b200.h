@@ -306,9 +306,10 @@ int exn_attn_open(int device, exn_attn** out);
 void exn_attn_close(exn_attn* a);
 const char* exn_attn_last_error(const exn_attn* a);
 
-/* Wait for STREAM and report what the kernels of this handle found wrong since the last such call:
- * EXN_EINVAL for bad offsets, lengths or pages, EXN_ETIMEOUT for a kernel that gave up (the outputs of the
- * calls since then hold anything, and a workspace that a captured call uses is to be zeroed). */
+/* Wait for STREAM and report what the kernels of this handle, on any stream, found wrong and no such call has
+ * reported yet: EXN_ETIMEOUT for a kernel that gave up (the outputs of the calls since then hold anything, and
+ * a workspace that a captured call uses is to be zeroed), whatever else was wrong; EXN_EINVAL for bad offsets,
+ * lengths or pages.  Not while STREAM is being captured. */
 int exn_attn_sync(exn_attn* a, void* stream);
 
 /* Causal attention of NSEQ packed sequences: q and out ROWS x heads * 128, k and v KV_ROWS x kv_heads *

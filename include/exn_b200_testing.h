@@ -164,6 +164,9 @@ int exn_test_enc_last_ms(const exn_enc* e, double* ms);
  * matrices, the fp32 vectors and embedding table), to compare two loads. */
 int exn_test_enc_weights_digest(exn_enc* e, uint64_t* out);
 
+/* What exn_attn_sync returns for the kernels' status word STATUS, and its message in TEXT (N bytes). */
+int exn_test_attn_report(int status, char* text, int n);
+
 #ifdef __cplusplus
 }
 #endif

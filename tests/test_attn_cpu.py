@@ -50,3 +50,13 @@ def test_kv_cache_has_the_headers_layout(tmp_path):
     subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", exe, str(src)], check=True)
     got = [int(x) for x in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [getattr(E.KvCache, n).offset for n in names] + [ctypes.sizeof(E.KvCache)]
+
+
+@pytest.mark.parametrize("status,code,words", [
+    (0, 0, []), (4, 1, ["offsets", "left them out"]), (2, 6, ["gave up", "0x2"]), (6, 6, ["gave up", "out of range"]),
+    (8, 6, ["gave up"])])
+def test_a_kernel_that_gave_up_is_reported_before_anything_else(status, code, words):
+    text = ctypes.create_string_buffer(512)
+    assert E.lib().exn_test_attn_report(status, text, len(text)) == code
+    assert all(w in text.value.decode() for w in words)
+    assert (code == 1) == ("left them out" in text.value.decode())

@@ -122,3 +122,28 @@ def test_cache_calls_with_offsets_that_decrease(att, bad, good):
                             heads, kv_heads)
             check(out[at[s]:at[s + 1]], ref, "bf16", p16="same" if c.dense else "fp16")
         assert (whole[:128] == 7).all() and (whole[-128:] == 7).all() and (out[at[good]:] == 7).all()
+
+
+def test_what_a_kernel_on_another_stream_finds_is_reported_once(att):
+    """Syncs on one stream while a bad call waits behind slow work on another: one of them, or the sync of
+    that stream, reports it, and one only."""
+    q, k, v = rows(64, 8, 1, "bf16"), rows(64, 2, 2, "bf16"), rows(64, 2, 3, "bf16")
+    out = torch.zeros_like(q)
+    bad = torch.tensor([0, 65], dtype=torch.int32, device="cuda")
+    slow, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(20):
+        big = torch.randn(2048, 2048, device="cuda")
+        torch.cuda.synchronize()
+        with torch.cuda.stream(slow):
+            for _ in range(3):
+                big = big @ big * 1e-3
+            att.packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), bad.data_ptr(), 1, 64, 8, 2,
+                       stream=slow.cuda_stream)
+        reports = 0
+        for st in [other] * 30 + [slow, other]:
+            try:
+                att.sync(st.cuda_stream)
+            except E.ExnError as e:
+                assert e.code == 1
+                reports += 1
+        assert reports == 1
