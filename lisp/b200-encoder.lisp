@@ -173,7 +173,11 @@
   (%enc-cache-close cache))
 
 (defun extend-prompts (model cache tokens)
-  "More tokens of every prompt of CACHE, a list of lists of ids (NIL: none): their states."
+  "More tokens of every prompt of CACHE, a list of as many lists of ids (NIL: none): their states."
+  ;; the library reads a count for every prompt that the cache was opened with
+  (let ((n (length tokens)))
+    (unless (and (plusp n) (>= (prompt-length cache (1- n)) 0) (minusp (prompt-length cache n)))
+      (error "extend-prompts: ~D lists of tokens, the cache has another number of prompts" n)))
   (call-on-prompts model tokens
                    (lambda (ids counts states)
                      (%enc-extend (genc-handle model) cache ids counts (sb-sys:int-sap 0) states))))

@@ -160,3 +160,53 @@ def test_encoder_driver_keeps_the_reference_lambda_lists():
     assert defuns["encoder-states"] == ["model", "ids", "&key", "rope"]
     assert defuns["mrope-table"] == ["positions", "rd", "base"]
     assert defuns["encoder-gpu-p"] == ["model"]
+
+
+# --------------------------------------------------------------------------- a small evaluator
+
+class LispError(Exception):
+    pass
+
+
+def run_lisp(form, env):
+    """The value of FORM, for the few operators that a function's argument checks use; ENV maps names to
+    values and to Python functions."""
+    if isinstance(form, str):
+        if form.startswith('"'):
+            return form.strip('"')
+        return int(form) if re.fullmatch(r"-?\d+", form) else env[form]
+    op, args = form[0], form[1:]
+    if op in ("let", "let*"):
+        env = dict(env)
+        for name, value in args[0]:
+            env[name] = run_lisp(value, env)
+        return [run_lisp(f, env) for f in args[1:]][-1]
+    if op == "lambda":
+        return lambda *given: [run_lisp(f, dict(env, **dict(zip(args[0], given)))) for f in args[1:]][-1]
+    if op == "unless":
+        return None if run_lisp(args[0], env) else [run_lisp(f, env) for f in args[1:]][-1]
+    if op == "and":
+        return all(run_lisp(a, env) for a in args)
+    if op == "error":
+        raise LispError([run_lisp(a, env) for a in args])
+    given = [run_lisp(a, env) for a in args]
+    plain = {"plusp": lambda x: x > 0, "minusp": lambda x: x < 0, ">=": lambda x, y: x >= y, "1-": lambda x: x - 1,
+             "length": len}
+    return (env.get(op) or plain[op])(*given)
+
+
+def test_extend_prompts_takes_a_list_for_every_prompt():
+    """exn_enc_extend reads as many counts as the cache has prompts, so another number of lists is an error."""
+    defun = next(f for f in forms(LISP_ENC) if f[0] == "defun" and f[1] == "extend-prompts")
+    assert defun[2] == ["model", "cache", "tokens"]
+    for prompts in (1, 3):
+        for lists in range(6):
+            calls = []
+            env = {"model": "m", "cache": "c", "tokens": [[1, 2]] * lists,
+                   "prompt-length": lambda c, s: 7 * s if 0 <= s < prompts else -1,
+                   "call-on-prompts": lambda m, t, f: calls.append(t) or "states"}
+            try:
+                value = [run_lisp(f, env) for f in defun[3:]][-1]
+                assert lists == prompts and value == "states" and len(calls) == 1
+            except LispError:
+                assert lists != prompts and not calls
