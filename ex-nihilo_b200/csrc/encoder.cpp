@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -74,6 +75,7 @@ struct EncLayer {
 };
 
 struct exn_enc {
+  uint64_t id = 0;  // no other encoder of the process has or had it
   exn_enc_config cfg{};
   int sms = 0, fit[3] = {0, 0, 0};  // packed_prepare's
   cudaStream_t st = nullptr;
@@ -103,7 +105,7 @@ struct exn_enc {
 // Kept keys and values of nseq sequences, every block's: the 8-bit cache of attn_cache.cu with a pool of
 // pages a block, sequence s's the pages s * ld .. s * ld + ld - 1
 struct exn_enc_cache {
-  exn_enc* owner = nullptr;
+  uint64_t owner = 0;  // the encoder's id: its address may be another's once it is closed
   int device = 0, nseq = 0, ld = 0, layers = 0, kv_heads = 0;
   int8_t* codes = nullptr;  // [layer][k, v][pages][kv_heads][64][128]
   float* scales = nullptr;  // [layer][k, v][pages][kv_heads]
@@ -574,7 +576,9 @@ int exn_enc_open(const exn_enc_config* cfg, exn_enc** out) {
   if (prop.major != 10)
     return efail(nullptr, EXN_EUNSUPPORTED, "exn_enc_open: device %d is sm_%d%d; this library is built for sm_100a",
                  c.device, prop.major, prop.minor);
+  static std::atomic<uint64_t> encoders{0};
   e = new exn_enc();
+  e->id = ++encoders;
   e->cfg = c;
   e->sms = prop.multiProcessorCount;
   const int rc = [&]() -> int {
@@ -960,7 +964,7 @@ int exn_enc_cache_open(exn_enc* e, int nseq, int max_tokens, exn_enc_cache** out
   ECK(cudaSetDevice(e->cfg.device));
   exn_enc_cache* c = new (std::nothrow) exn_enc_cache();
   if (!c) return efail(e, EXN_ENOMEM, "exn_enc_cache_open: out of memory");
-  c->owner = e;
+  c->owner = e->id;
   c->device = e->cfg.device;
   c->nseq = nseq;
   c->ld = static_cast<int>(ld);
@@ -997,7 +1001,7 @@ void exn_enc_cache_close(exn_enc_cache* c) {
 int exn_enc_cache_length(const exn_enc_cache* c, int seq) { return c && seq >= 0 && seq < c->nseq ? c->lens[seq] : -1; }
 
 int exn_enc_cache_trim(exn_enc* e, exn_enc_cache* c, int seq, int tokens) {
-  if (!e || !c || c->owner != e) return efail(e, EXN_EINVAL, "exn_enc_cache_trim: null argument, or another encoder's cache");
+  if (!e || !c || c->owner != e->id) return efail(e, EXN_EINVAL, "exn_enc_cache_trim: null argument, or another encoder's cache");
   if (seq < 0 || seq >= c->nseq || tokens < 0 || tokens > c->lens[seq])
     return efail(e, EXN_EINVAL, "exn_enc_cache_trim: sequence %d of %d to %d tokens of %d", seq, c->nseq, tokens,
                  seq >= 0 && seq < c->nseq ? c->lens[seq] : 0);
@@ -1007,7 +1011,7 @@ int exn_enc_cache_trim(exn_enc* e, exn_enc_cache* c, int seq, int tokens) {
 
 int exn_enc_extend(exn_enc* e, exn_enc_cache* c, const int32_t* ids, const int32_t* counts, const int32_t* positions,
                    float* states) {
-  if (!e || !c || c->owner != e) return efail(e, EXN_EINVAL, "exn_enc_extend: null argument, or another encoder's cache");
+  if (!e || !c || c->owner != e->id) return efail(e, EXN_EINVAL, "exn_enc_extend: null argument, or another encoder's cache");
   static const char fn[] = "exn_enc_extend";
   return guarded(e, fn, [&] { return run_sequences(e, fn, c, ids, c->nseq, counts, positions, 0, states, false, nullptr); });
 }

@@ -258,9 +258,9 @@ int exn_enc_states_packed_device(exn_enc* e, const int32_t* ids, int nseq, const
 /* Prompts that grow: the keys and values of NSEQ sequences of up to MAX_TOKENS tokens (rounded up to a
  * multiple of 64) are kept in 8 bits (the cache of exn_attn_cache_write below, every block's), so that a
  * token is encoded once: the system turn that every prompt starts with, a prompt that is edited from some
- * word on.  The cache belongs to the encoder it was opened on, is used by one thread at a time with it,
- * and may be closed before or after it.  Its memory: 2 * layers * kv_heads * 128 bytes a token (73.7 KB
- * for Qwen3-VL-8B). */
+ * word on.  The cache belongs to the encoder it was opened on (another one refuses it), is used by one
+ * thread at a time with it, and may be closed before or after it.  Its memory: 2 * layers * kv_heads * 128
+ * bytes a token (73.7 KB for Qwen3-VL-8B). */
 typedef struct exn_enc_cache exn_enc_cache;
 int exn_enc_cache_open(exn_enc* e, int nseq, int max_tokens, exn_enc_cache** out);
 void exn_enc_cache_close(exn_enc_cache* c);

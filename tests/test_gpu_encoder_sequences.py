@@ -196,3 +196,29 @@ def test_refusals(small):
         with pytest.raises(E.ExnError) as e:
             bare.states_packed([[1]])
         assert e.value.code == 4
+
+
+def test_a_cache_of_a_closed_encoder_is_refused(small):
+    """Another encoder, which may have got the closed one's address, does not take its cache."""
+    first = E.Encoder(**SMALL)
+    cache = first.cache(2, 64)
+    address = first.h.value
+    first.close()
+    others = []
+    for _ in range(8):
+        others.append(E.Encoder(**SMALL))
+        if others[-1].h.value == address:
+            break
+    for other in others + [small]:
+        other.load_synthetic(1)
+        cache.encoder = other
+        with pytest.raises(E.ExnError) as e:
+            cache.trim(0, 0)
+        assert e.value.code == 1 and "another encoder" in str(e.value)
+        with pytest.raises(E.ExnError) as e:
+            cache.extend([[1], [2, 3]])
+        assert e.value.code == 1 and "another encoder" in str(e.value)
+    assert cache.lengths() == [0, 0]
+    cache.close()
+    for other in others:
+        other.close()
