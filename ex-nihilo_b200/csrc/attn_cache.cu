@@ -52,6 +52,9 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
+// 2^e of a whole number -127 (0 then) .. 127: its exponent is in the low bits of a float whose unit is 1
+__device__ __forceinline__ float pow2_of(float e) { return __uint_as_float(__float_as_uint(e + 0x1.8000fep23f) << 23); }
+
 __device__ __forceinline__ int to_code(float x, float top) { return __float2int_rn(fminf(fmaxf(x, -top), top)); }
 
 // The rows of a call that fall into one page, by the page's slot: sequence s owns the slots from
@@ -289,10 +292,12 @@ __global__ void __launch_bounds__(128) k_cache_read(const CacheArgs c, const int
 //     itself is, for elements of 1/128 (bf16) or 1/16 (fp16) of the row's largest and more, and off by
 //     at most 2^-15 of the largest below;
 //   * V's codes become fp16 (m16n8k16), exactly: ldmatrix.trans brings a position pair's codes of two
-//     dims into one register, from which 1024 + (code + 128) is 0x6400 | byte; the subtraction of 1152 is a
-//     fused multiply-add that scales by 2^ev as well, relative to the unit the warp's sums are in, so
-//     the product adds to the sums in place.  P is fp16, at most 2^8: the sums are rescaled only
-//     when the row maximum grows by more than 2^8;
+//     dims into one register, from which 1024 + (code + 128) is 0x6400 | byte, less 1152;
+//   * what multiplies them is P' = P 2^(ev - u) in fp16, P the fp32 softmax weight, 2^ev the page's scale and
+//     2^u the unit of the row's sums, a power of two that follows the row's largest P 2^ev: P' stays
+//     between 1 and 2^14 for it, so what fp16 drops (P' < 2^-25) is 2^-25 of the row's largest product of a
+//     weight and a scale, whatever the scales of the pages are.  The sums are rescaled only when the row
+//     maximum grows by more than 2^8 or P' would leave that range;
 //   * P^T turns from the first product's layout to the second's with movmatrix.
 constexpr int SPAN = 32;                  // positions a warp takes at a time
 constexpr int SPAN_BYTES = SPAN * 128;
@@ -332,10 +337,10 @@ __device__ __forceinline__ void mma16832(int (&c)[4], uint32_t a0, uint32_t a1, 
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// two of four biased codes (code + 128), bytes 0 and 2 or 1 and 3, as fp16 code * r: (1024 + byte) r - 1152 r, exact
-__device__ __forceinline__ uint32_t v_pair(uint32_t u, uint32_t sel, __half2 r, __half2 c) {
+// two of four biased codes (code + 128), bytes 0 and 2 or 1 and 3, as fp16: 1024 + byte - 1152, exact
+__device__ __forceinline__ uint32_t v_pair(uint32_t u, uint32_t sel) {
   const uint32_t h = __byte_perm(u, 0x64646464u, sel);
-  const __half2 x = __hfma2(*reinterpret_cast<const __half2*>(&h), r, c);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&x);
 }
 constexpr uint32_t EVEN = 0x4240, ODD = 0x4341;
@@ -852,20 +857,18 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
         lim[nt][j] = row < nrows ? pos0 + row / nh : -1;
       }
 
-    float m[NT][2], l[NT][2], o[NT][8][4];
+    // a row's maximum and sum of weights; log2 of its largest P 2^ev so far over 2^m (top) and of its sums' unit
+    // (unit, an integer)
+    float m[NT][2], l[NT][2], top[NT][2], unit[NT][2], o[NT][8][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+      m[nt][0] = m[nt][1] = top[nt][0] = top[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = unit[nt][0] = unit[nt][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
     }
-    // V's unit: o is in multiples of UNIT; codes of a page of scale sv are multiplied by sv / UNIT while
-    // that is an exact fp16 factor (2^-24 .. 2^5 of codes up to 127), else the unit changes
-    float unit = 0.f, vscale = 0.f;
-    __half2 vr = __half2half2(__ushort_as_half(0)), vb = vr;
     for (; turn < n; turn += WARPS) {
       ok = mbar_wait_uniform(&full[slot], phase, abort_flag, status, STATUS_TIMEOUT_ATTN);
       if (!ok) break;
@@ -908,11 +911,12 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
       step();
       // softmax: one running maximum and sum a query row and warp
       const bool masked = pos + SPAN - 1 > pos0;  // past the last position that every row sees
+      const float ev = static_cast<float>((__float_as_int(svp) >> 23) - 127);  // V's scale is 2^ev
       uint32_t pf[NT][2][2];
       float s[NT][2][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float alpha[2];
+        float grown[2];  // how far the maximum grows
         bool need = false;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -931,21 +935,31 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           const bool grow = mx > m[nt][j] + 8.f;
-          alpha[j] = grow ? fast_exp2(m[nt][j] - mx) : 1.f;
+          grown[j] = grow ? mx - m[nt][j] : 0.f;
           m[nt][j] = grow ? mx : m[nt][j];
-          need |= grow;
+          const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];  // nothing seen yet: every P is 2^-inf = 0
+          top[nt][j] = fmaxf(top[nt][j] - grown[j], mx - mu + ev);
+          const float above = top[nt][j] - unit[nt][j];
+          need |= grow || above > 14.f || (above < 0.f && top[nt][j] > -INFINITY);
         }
         if (__any_sync(0xffffffffu, need)) {
+          float f[2];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) l[nt][j] *= alpha[j];
+          for (int j = 0; j < 2; ++j) {
+            const float above = top[nt][j] - unit[nt][j], before = unit[nt][j];
+            if (above > 14.f || (above < 0.f && top[nt][j] > -INFINITY)) unit[nt][j] = fminf(floorf(top[nt][j]), 127.f);
+            f[j] = fast_exp2(before - unit[nt][j] - grown[j]);  // at most 2: TOP fell by no more than the maximum grew
+            l[nt][j] *= fast_exp2(-grown[j]);
+          }
 #pragma unroll
           for (int q = 0; q < 8; ++q)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[nt][q][j] *= alpha[j & 1];
+            for (int j = 0; j < 4; ++j) o[nt][q][j] *= f[j & 1];
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];  // nothing seen yet: every P is 2^-inf = 0
+          const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];
+          const float to_unit = pow2_of(fminf(fmaxf(ev - unit[nt][j], -127.f), 127.f));
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -953,6 +967,7 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
               float& x = s[nt][mt][2 * hh + j];
               x = fast_exp2(x - mu);
               l[nt][j] += x;
+              x *= to_unit;
             }
         }
 #pragma unroll
@@ -961,49 +976,14 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
           for (int hh = 0; hh < 2; ++hh)
             pf[nt][mt][hh] = transpose8x8(pack16<true>(s[nt][mt][2 * hh], s[nt][mt][2 * hh + 1]));
       }
-      if (svp != vscale) {  // the same for the whole warp
-        vscale = svp;
-        float r = svp / unit;  // a ratio of powers of two
-        if (svp != svp) {      // a page of scale NaN: the rows that see a position of it are NaN
+      if (svp != svp) {  // a page of scale NaN: the rows that see a position of it are NaN
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
+          for (int q = 0; q < 8; ++q)
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (pos <= lim[nt][j & 1]) o[nt][q][j] = svp;
-          r = 0.f;
-          vscale = 0.f;  // for the next page of its kind
-        } else if (svp == 0.f) {
-          r = 0.f;
-        } else if (!(r >= 0x1p-24f && r <= 32.f)) {
-          float big = 0.f;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) big = fmaxf(big, fabsf(o[nt][q][j]));
-#pragma unroll
-          for (int x = 16; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-          const float change = unit / svp;
-          if (big > 0.f && big * change > 0x1p100f) {
-            r = 0.f;  // 2^-60 of what the sums hold: it adds nothing to them
-            vscale = 0.f;
-          } else {
-            if (big > 0.f)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-#pragma unroll
-                  for (int j = 0; j < 4; ++j) o[nt][q][j] *= change;
-            unit = svp;
-            r = 1.f;
-          }
-        }
-        vr = __float2half2_rn(r);
-        vb = __float2half2_rn(-1152.f * r);
+            for (int j = 0; j < 4; ++j)
+              if (pos <= lim[nt][j & 1]) o[nt][q][j] = svp;
       }
       ok = mbar_wait_uniform(&full[slot], phase, abort_flag, status, STATUS_TIMEOUT_ATTN);
       if (!ok) break;
@@ -1022,8 +1002,7 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               const uint32_t x = w[q >> 1][2 * z] ^ 0x80808080u, y = w[q >> 1][2 * z + 1] ^ 0x80808080u;
-              const uint32_t fr[4] = {v_pair(x, EVEN, vr, vb), v_pair(x, ODD, vr, vb), v_pair(y, EVEN, vr, vb),
-                                      v_pair(y, ODD, vr, vb)};
+              const uint32_t fr[4] = {v_pair(x, EVEN), v_pair(x, ODD), v_pair(y, EVEN), v_pair(y, ODD)};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][q + z], fr, pf[nt][mt][0], pf[nt][mt][1]);
             }
@@ -1043,6 +1022,7 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
         t += __shfl_xor_sync(0xffffffffu, t, 8);
         t += __shfl_xor_sync(0xffffffffu, t, 16);
         const int row = nt * 8 + 2 * ti + j;
+        const float u = pow2_of(unit[nt][j]);
         if (gi == 0) {
           sh.m[warp][row] = m[nt][j];
           sh.l[warp][row] = t;
@@ -1050,7 +1030,7 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           *reinterpret_cast<float2*>(&part_o[warp][row][16 * q + 2 * gi]) =
-              make_float2(o[nt][q][j] * unit, o[nt][q][j + 2] * unit);
+              make_float2(o[nt][q][j] * u, o[nt][q][j + 2] * u);
       }
     const Seg seg = sh.seg[b];
     const int part_len = sh.part_len, lead = sh.lead;

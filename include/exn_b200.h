@@ -282,8 +282,11 @@ int exn_enc_release(exn_enc* e);
  * for programs that keep their own activations or caches on the GPU.  No counterpart in the reference,
  * which encodes one prompt a call and keeps nothing (src/encoder.lisp:143-183).
  *
- * Head dimension 128.  TYPE is EXN_GGML_BF16 or EXN_GGML_F16, the type of q, k, v and the outputs; sums,
- * maxima and the softmax are fp32.  Query head h reads key/value head h / (heads / kv_heads), heads a
+ * Head dimension 128.  TYPE is EXN_GGML_BF16 or EXN_GGML_F16, the type of q, k, v and the outputs.  Scores,
+ * maxima, the softmax's weights and all sums are fp32; what multiplies a value is its weight in 16 bits: in
+ * TYPE, where fp16 drops weights below 2^-25 of the row's largest, or, in cached attention of few rows, in
+ * fp16 relative to the row's largest product of a weight and a page's scale, of which it drops what is below
+ * 2^-25.  Query head h reads key/value head h / (heads / kv_heads), heads a
  * multiple of kv_heads and at most 128 times it.  Every pointer but the handle's and *CACHE itself is
  * device memory of the handle's device.  Rows are packed: row r of a matrix starts at r * ld elements,
  * its heads side by side; ld a multiple of 8 (0: the rows are contiguous), bases 16-byte aligned.

@@ -147,3 +147,123 @@ def test_what_a_kernel_on_another_stream_finds_is_reported_once(att):
                 assert e.code == 1
                 reports += 1
         assert reports == 1
+
+
+# --------------------------------------------------------------------------- pages of values of very different sizes
+
+
+def pages_of_sizes(t, heads, kv_heads, v_exponents, k_levels, seed, few=0):
+    """A cache of one sequence whose page i has values of the size 2^v_exponents[i] and keys whose scores are
+    about k_levels[i] (natural logarithms), and rows of q; all numbers small multiples of powers of two, so
+    that the cache holds them exactly and the scores' sums are exact.  The last page has FEW positions (0: all)."""
+    n = 64 * len(v_exponents) - (64 - few if few else 0)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    side = torch.randint(0, 2, (1, 1, D), generator=g, device="cuda") * 2.0 - 1
+    q = side.expand(1, heads, D) * torch.tensor([1.0, 0.5, 1.0, 2.0], device="cuda").repeat(heads)[:heads, None]
+    page = torch.arange(n, device="cuda") // 64
+    # side . k = 128 level: the score is level * 128 / sqrt(128); one more key dim turned over changes it a little
+    level = torch.tensor([round(x * 64 / 11.3137) / 64 for x in k_levels], device="cuda")[page]
+    turned = torch.rand(n, kv_heads, D, generator=g, device="cuda") < 0.02
+    k = level[:, None, None] * side * torch.where(turned, -1.0, 1.0)
+    size = torch.exp2(torch.tensor([float(x) for x in v_exponents], device="cuda"))[page]
+    v = torch.randint(-96, 97, (n, kv_heads, D), generator=g, device="cuda") * size[:, None, None]
+    c = Cache(1, len(v_exponents), kv_heads)
+    return c, [x.to(TYPES[t]).reshape(len(x), -1) for x in (q, k, v)]
+
+
+def check_wide(out, c, q, heads, kv_heads, t, p_step):
+    """As check of test_gpu_attn.py, with what the weights' 16 bits drop measured by the row's largest product
+    of a weight and a page's scale: each of N positions loses a code of up to 127 times 2^-25 of it."""
+    v = c.model[0]["v"].cuda()
+    n = v.shape[0]
+    o, a, _ = reference(q, c.model[0]["k"].cuda().flatten(1), v.flatten(1), heads, kv_heads)
+    scales = torch.tensor([[2.0 ** c.units[0]["v"][j // 64, h] for h in range(kv_heads)] for j in range(n)], device="cuda").double()
+    w = reference(q, c.model[0]["k"].cuda().flatten(1), scales[:, :, None].expand(n, kv_heads, D).flatten(1), heads, kv_heads)
+    # w[0] is the sum of weights times scales, at least the largest of them
+    tol = 2 ** -8 * o.abs() if t == "bf16" else 2 ** -11 * o.abs() + 2.0 ** -25
+    tol = tol + (p_step + 2 ** -11.5) * a + n * 127 * 2.0 ** -25 * w[0]
+    assert torch.isfinite(out).all()
+    worst = ((out.double() - o).abs() / tol).max().item()
+    assert worst <= 1, "an output is %.3g of its bound off" % worst
+
+
+def attend_copies(att, c, q, heads, t, copies):
+    """c's attention for COPIES sequences of the same pages, [copies][rows of q]: so many items that a warp
+    takes several pages of each."""
+    n = q.shape[0]
+    table, lens = c.table[:1].repeat(copies, 1), c.lens[:1].repeat(copies)
+    one = E.KvCache.from_buffer_copy(c.c)
+    one.nseq, one.table, one.lens = copies, table.data_ptr(), lens.data_ptr()
+    o = offsets([n] * copies)
+    qs = q.repeat(copies, 1)
+    out = torch.full_like(qs, 7.0)
+    space = torch.empty(att.cache_workspace(one, n * copies, heads), dtype=torch.uint8, device="cuda")
+    att.cache_attend(one, qs.data_ptr(), out.data_ptr(), o.data_ptr(), n * copies, heads, dtype=GGML[t],
+                     workspace=space.data_ptr(), workspace_bytes=space.numel())
+    att.sync()
+    assert n * (heads // c.kv) <= 64  # the kernel that reads the codes
+    return out.reshape(copies, n, heads * D)
+
+
+WIDE = [  # sizes of the pages' values and levels of their scores
+    ([0, 30], [20, 0]),                  # a weight of 2^-29 on values 2^30 times as large
+    ([0] * 9 + [30] * 9, [20] * 9 + [0] * 9),
+    ([30] * 9 + [0] * 9, [0] * 9 + [20] * 9),
+    ([0, 34, 0, 33] * 5, [23, 0, 22, 1] * 5),
+    ([-60] * 7 + [60] * 7, [0] * 14),    # the larger pages are the output, in either order
+    ([60] * 7 + [-60] * 7, [0] * 14),
+    ([-40, -80, -60, 10, -50, -41] * 4, [30, 60, 45, 0, 38, 31] * 4),
+    ([100] * 6 + [-100] * 6 + [0] * 6, [0] * 6 + [80] * 6 + [40] * 6),  # as far apart as bf16 allows
+    ([7 * (i % 9) - 30 for i in range(40)], [1.5 * (i % 7) for i in range(40)]),
+]
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(4, 1), (8, 2), (16, 1)])
+@pytest.mark.parametrize("sizes,levels", WIDE)
+@pytest.mark.parametrize("few,copies", [(0, 1), (5, 1), (40, 400)])
+def test_attention_over_pages_of_very_different_sizes(att, heads, kv_heads, sizes, levels, few, copies):
+    """A small weight on large values counts as much as a large one on small values, whichever page comes
+    first, in one warp or in several."""
+    c, (q, k, v) = pages_of_sizes("bf16", heads, kv_heads, sizes, levels, 1, few)
+    c.write(att, [k.shape[0]], k, v, "bf16")
+    out = attend_copies(att, c, q, heads, "bf16", copies)
+    check_wide(out[:, 0], c, q, heads, kv_heads, "bf16", 2 ** -11)
+    assert torch.equal(out, attend_copies(att, c, q, heads, "bf16", copies))
+
+
+def test_one_token_and_a_chunk_agree_over_pages_of_different_sizes(att):
+    """The same rows by either path of cached attention."""
+    heads, kv_heads = 8, 2
+    c, (q, k, v) = pages_of_sizes("bf16", heads, kv_heads, [0, 30, 1, 31] * 4, [20, 0, 19, 1] * 4, 2)
+    c.write(att, [k.shape[0]], k, v, "bf16")
+    one = attend_copies(att, c, q, heads, "bf16", 400)[:, 0]
+    many = q.repeat(40, 1)
+    chunk = c.attend(att, [40], many, heads, "bf16")
+    assert c.dense
+    check_wide(one, c, q, heads, kv_heads, "bf16", 2 ** -11)
+    check_wide(chunk[-1:], c, q, heads, kv_heads, "bf16", 2 ** -8)
+
+
+def test_rows_of_a_tile_keep_their_own_unit(att):
+    """Rows that share a tile and see different pages: the ones that a page of huge values is hidden from, or
+    has no weight for, keep theirs."""
+    heads, kv_heads = 4, 1
+    c, (q, k, v) = pages_of_sizes("bf16", heads, kv_heads, [-100] * 8 + [20], [0] * 9, 3, few=2)
+    # the last two positions have huge values; row 0 sees neither, row 1 the first, row 2 both
+    c.write(att, [k.shape[0]], k, v, "bf16")
+    for copies in (1, 400):
+        out = attend_copies(att, c, q.repeat(3, 1), heads, "bf16", copies)
+        check_wide(out[:, 2], c, q, heads, kv_heads, "bf16", 2 ** -11)
+        c.lens -= 2
+        model, c.model[0]["v"] = c.model[0]["v"], c.model[0]["v"][:-2]
+        keys, c.model[0]["k"] = c.model[0]["k"], c.model[0]["k"][:-2]
+        check_wide(out[:, 0], c, q, heads, kv_heads, "bf16", 2 ** -11)
+        c.lens += 2
+        c.model[0] = dict(k=keys, v=model)
+    # a head that turns away from the huge pages: scores of -100, weights of 2^-144 times values of 2^120 times as large
+    for sizes in ([-100] * 8 + [20] * 8, [20] * 8 + [-100] * 8):
+        c, (q, k, v) = pages_of_sizes("bf16", heads, kv_heads, sizes, [25 * (x > 0) for x in sizes], 4)
+        c.write(att, [k.shape[0]], k, v, "bf16")
+        q[:, D:2 * D] *= -8
+        for copies in (1, 400):
+            check_wide(attend_copies(att, c, q, heads, "bf16", copies)[:, 0], c, q, heads, kv_heads, "bf16", 2 ** -11)
