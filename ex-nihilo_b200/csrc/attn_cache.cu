@@ -289,8 +289,9 @@ __global__ void __launch_bounds__(128) k_cache_read(const CacheArgs c, const int
 //     rows of queries waste nothing;
 //   * K's codes are multiplied as they are (m16n8k32, s8): a row of q is two int8 numbers, q = 2^a (hi +
 //     lo / 256) with 2^a the smallest power of two that |q| <= 127 2^a allows.  The sums are exact; q
-//     itself is, for elements of 1/128 (bf16) or 1/16 (fp16) of the row's largest and more, and off by
-//     at most 2^-15 of the largest below;
+//     itself is, for elements of 1/128 (bf16) or 1/16 (fp16) of the row's largest M and more, and off by
+//     at most 2^a / 512 <= M / 32512 below.  Over 128 codes of up to 127 that moves a score by no more than M / 2
+//     of K's scale, which is what K's own rounding may do in one element;
 //   * V's codes become fp16 (m16n8k16), exactly: ldmatrix.trans brings a position pair's codes of two
 //     dims into one register, from which 1024 + (code + 128) is 0x6400 | byte, less 1152;
 //   * what multiplies them is P' = P 2^(ev - u) in fp16, P the fp32 softmax weight, 2^ev the page's scale and
@@ -444,9 +445,9 @@ __device__ __forceinline__ void put_query(AttendShared<NT>& sh, int b, int r, ui
   uint32_t hi[4], lo[4];  // in the low bits of floats near 1.5 * 2^23, whose unit is 1
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float x = v[i] * inv, h = __fadd_rd(x + 0.5f, 0x1.8p23f);  // halves up: lo = -128 there
+    const float x = v[i] * inv, h = __fadd_rd(x + 0x1.01p-1f, 0x1.8p23f);  // hi: lo is then -128 .. 127 without a clamp
     hi[i] = __float_as_uint(h);
-    lo[i] = __float_as_uint(fminf(fmaf(x - (h - 0x1.8p23f), 256.f, 0x1.8p23f), 0x1.8p23f + 127.f));
+    lo[i] = __float_as_uint(fmaf(x - (h - 0x1.8p23f), 256.f, 0x1.8p23f));
   }
   sh.q[b][0][r][lane] = __byte_perm(__byte_perm(hi[0], hi[1], 0x0040), __byte_perm(hi[2], hi[3], 0x0040), 0x5410);
   sh.q[b][1][r][lane] = __byte_perm(__byte_perm(lo[0], lo[1], 0x0040), __byte_perm(lo[2], lo[3], 0x0040), 0x5410);

@@ -286,7 +286,7 @@ int exn_enc_release(exn_enc* e);
  * maxima, the softmax's weights and all sums are fp32; what multiplies a value is its weight in 16 bits: in
  * TYPE, where fp16 drops weights below 2^-25 of the row's largest, or, in cached attention of few rows, in
  * fp16 relative to the row's largest product of a weight and a page's scale, of which it drops what is below
- * 2^-25.  Query head h reads key/value head h / (heads / kv_heads), heads a
+ * 2^-25; there q's small elements are rounded too, by at most 1 / 32512 of their row and head's largest.  Query head h reads key/value head h / (heads / kv_heads), heads a
  * multiple of kv_heads and at most 128 times it.  Every pointer but the handle's and *CACHE itself is
  * device memory of the handle's device.  Rows are packed: row r of a matrix starts at r * ld elements,
  * its heads side by side; ld a multiple of 8 (0: the rows are contiguous), bases 16-byte aligned.

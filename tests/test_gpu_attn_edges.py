@@ -267,3 +267,37 @@ def test_rows_of_a_tile_keep_their_own_unit(att):
         q[:, D:2 * D] *= -8
         for copies in (1, 400):
             check_wide(attend_copies(att, c, q, heads, "bf16", copies)[:, 0], c, q, heads, kv_heads, "bf16", 2 ** -11)
+
+
+@pytest.mark.parametrize("t,fraction", [("fp16", 0.5 - 2 ** -12), ("fp16", 0.5 + 2 ** -10), ("bf16", 0.5 - 2 ** -9),
+                                        ("fp16", -0.5 + 2 ** -12), ("fp16", 1.5 - 2 ** -10), ("fp16", -63.5 + 2 ** -5)])
+def test_small_query_elements_are_rounded_to_nearest(att, t, fraction):
+    """Rows of q of 127 equal elements beside one of 127, which no key sees: each of the 127 may be off by 1/512
+    (half of 1/256 of the unit 1), which moves a score of equal keys of 8 by 127 * 8 / 512 times the scale and,
+    between keys of 8 and of -8, a weight by twice that relatively."""
+    c = Cache(1, 3, 1)
+    k = torch.full((130, D), 8.0, device="cuda")
+    k[::2] *= -1
+    k[:, 5] = 0
+    v = torch.ones(130, D, dtype=TYPES[t], device="cuda")  # the output is the two kinds' weights' difference
+    v[::2] *= -1
+    q = torch.full((1, 2 * D), fraction, device="cuda")
+    q[0, 5] = 127
+    q[0, D + 5] = -127
+    q, k = q.to(TYPES[t]), k.to(TYPES[t])
+    assert q[0, 0].item() == fraction
+    c.write(att, [130], k, v, t)
+    scale = 2.0 ** -10 / max(1.0, abs(fraction))  # scores of about -1 .. 1: the weights stay of one size
+    out = torch.zeros_like(q)
+    o = offsets([1])
+    space = torch.empty(att.cache_workspace(c.c, 1, 2), dtype=torch.uint8, device="cuda")
+    att.cache_attend(c.c, q.data_ptr(), out.data_ptr(), o.data_ptr(), 1, 2, dtype=GGML[t], scale=scale,
+                     workspace=space.data_ptr(), workspace_bytes=space.numel())
+    att.sync()
+    ref, a, absv = reference(q, c.model[0]["k"].cuda().flatten(1), c.model[0]["v"].cuda().flatten(1), 2, 1, scale)
+    u = 2 ** -8 if t == "bf16" else 2 ** -11
+    err = max(abs(math.remainder(fraction, 1 / 256)), 2 ** -24)  # what the nearest multiple of 1/256 is off
+    assert err <= 1 / 512
+    tol = u * ref.abs() + 2.0 ** -25 + (2 ** -11 + 2 ** -11.5 + 2.1 * 127 * 8 * err * scale) * a + 2.0 ** -25 * absv
+    worst = ((out.double() - ref).abs() / tol).max().item()
+    assert worst <= 1, "an output is %.3g of its bound off" % worst
