@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(128) k_cache_write(const CacheArgs c, const in
   const float mine = pow2(scale_exponent(poisoned ? 0.f : amax));
   const float now = fmaxf(mine, before);
   const float inv = 1.f / now;  // exact: a power of two between 2^-122 and 2^126
-  const float top = now < 0x1p122f ? 127.f : 63.f;  // 64 * 2^122 would be infinite
+  const float top = now == (F16 ? 0x1p10f : 0x1p122f) ? 63.f : 127.f;  // 64 of the type's largest scale are infinite
   if (lo > 0 && !poisoned && now > before) {  // the codes that are there, in the larger unit
     const float f = before * inv;
 #pragma unroll

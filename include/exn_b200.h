@@ -327,7 +327,8 @@ int exn_attn_packed(exn_attn* a, int type, int heads, int kv_heads, int nseq, co
 /* Keys and values held in 8 bits, in pages of 64 positions.  A page has, for every key/value head, codes
  * int8 [64][128] and one scale, a power of two: the smallest >= 2^-126 with max |x| <= 127 scale over
  * what the page has held since its first position was last written; a value is code * scale, off by at
- * most scale / 2 when it is written and, after later tokens made the scale grow, by less than the scale.
+ * most scale / 2 when it is written (by less than the scale within 1/128 of TYPE's largest number, where the
+ * next code would be infinite) and, after later tokens made the scale grow, by less than the scale.
  * A page that is given an infinity or a NaN takes the scale NaN, and rows that see a position of it are
  * NaN, until its first position is written anew. */
 typedef struct exn_kv_cache {

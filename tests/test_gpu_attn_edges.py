@@ -301,3 +301,38 @@ def test_small_query_elements_are_rounded_to_nearest(att, t, fraction):
     tol = u * ref.abs() + 2.0 ** -25 + (2 ** -11 + 2 ** -11.5 + 2.1 * 127 * 8 * err * scale) * a + 2.0 ** -25 * absv
     worst = ((out.double() - ref).abs() / tol).max().item()
     assert worst <= 1, "an output is %.3g of its bound off" % worst
+
+
+# --------------------------------------------------------------------------- the largest numbers of a type
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_the_largest_numbers_stay_finite(att, t):
+    """Values up to the type's largest are held off by less than their scale, by at most half of it below 63.5
+    times it, and come back finite, by reading and by attention, also after a page's scale has grown to them."""
+    biggest = torch.finfo(TYPES[t]).max
+    unit = 2.0 ** (10 if t == "fp16" else 122)
+    x = torch.zeros(80, D, device="cuda")
+    x[:64] = torch.linspace(-1, 1, 64, device="cuda")[:, None] * biggest
+    x[64:72] = 0.49 * biggest  # a scale of half of UNIT, then the largest: it grows
+    x[72:76, ::2], x[76:] = biggest, -biggest
+    x = x.to(TYPES[t])
+    c = Cache(1, 2, 1)
+    for part in (x[:64], x[64:72], x[72:]):
+        c.lens += len(part)
+        o = offsets([len(part)])
+        att.cache_write(c.c, part.data_ptr(), part.data_ptr(), o.data_ptr(), len(part), dtype=GGML[t])
+        att.sync()
+    k, v = c.read(att, [80], t)
+    assert torch.equal(k, v) and torch.isfinite(k).all()
+    for page in (0, 1):
+        assert c.scales["k"][c.table[0, page], 0].item() == unit
+    off = (k.double() - x.double()).abs()
+    assert (off < unit).all() and (off[x.double().abs() <= 63.5 * unit] <= unit / 2).all()
+    zero = torch.zeros(1, D, dtype=TYPES[t], device="cuda")  # equal weights for all positions
+    c.lens.fill_(1)
+    out = c.attend(att, [1], zero, 1, t)
+    assert torch.equal(out[0], k[0])
+    many = torch.zeros(129, 1 * D, dtype=TYPES[t], device="cuda")
+    out = c.attend(att, [129], many, 1, t)
+    assert c.dense and torch.equal(out[-1], k[0])
