@@ -1196,13 +1196,13 @@ int cache_read_launch(const CacheArgs& c, int f16, const int* offsets, long long
                                      static_cast<uint16_t*>(k), ld_k, static_cast<uint16_t*>(v), ld_v, d_status));
 }
 
+static long long dense_blocks(const CacheArgs& c) { return static_cast<long long>(c.nseq) * c.table_ld * c.kv_heads * 2; }
 static int dense_launch(const CacheArgs& c, int f16, void* k, void* v, int* d_status, cudaStream_t st) {
-  const long long blocks = static_cast<long long>(c.nseq) * c.table_ld * c.kv_heads * 2;
-  if (blocks > 0x7fffffffll) return -1;
   const long long ld = static_cast<long long>(c.kv_heads) * 128;
   return static_cast<int>(launch_pdl(f16 ? k_cache_read<true, true> : k_cache_read<false, true>,
-                                     dim3(static_cast<unsigned>(blocks)), dim3(128), 0, st, c, static_cast<const int*>(nullptr),
-                                     0ll, static_cast<uint16_t*>(k), ld, static_cast<uint16_t*>(v), ld, d_status));
+                                     dim3(static_cast<unsigned>(dense_blocks(c))), dim3(128), 0, st, c,
+                                     static_cast<const int*>(nullptr), 0ll, static_cast<uint16_t*>(k), ld,
+                                     static_cast<uint16_t*>(v), ld, d_status));
 }
 
 int status_take_launch(int* status, cudaStream_t st) {
@@ -1226,11 +1226,12 @@ int cache_prepare() {
 //   1 sequence of 8000       23 / 37     31 / 37     32 / 37     42 / 37     54 / 40
 //   8 sequences of 2000      24 / 44     47 / 50     62 / 50     76 / 51    105 / 53
 //   32 sequences of 4000    130 / 245   236 / 246   339 / 248   443 / 252   657 / 269
-// so the bound is 64 rows a sequence and 64 more for the launch.
-static bool dense_path(const CacheArgs& c, int heads, long long rows) {
-  return rows * (heads / c.kv_heads) > 64 * (c.nseq + 1ll);
-}
+// so the bound is 64 rows a sequence and 64 more for the launch.  Tables with room for more positions than one
+// launch can turn into 16 bits leave the codes.
 static long long dense_rows(const CacheArgs& c) { return static_cast<long long>(c.nseq) * c.table_ld * kPage; }
+static bool dense_path(const CacheArgs& c, int heads, long long rows) {
+  return rows * (heads / c.kv_heads) > 64 * (c.nseq + 1ll) && dense_rows(c) <= 0x7fffffffll && dense_blocks(c) <= 0x7fffffffll;
+}
 
 // the cut of the direct path's work: a wave of CTAs, tiles of 8 or 16 query rows.  us with tiles of 8 / 16
 // (bf16; the codes are read again for every tile):
@@ -1288,7 +1289,6 @@ int cache_attention(const CacheAttnArgs& a, void* ws, size_t ws_bytes, int sms, 
   const CacheArgs& c = a.c;
   if (ws_bytes < cache_attention_workspace(c, a.heads, a.rows, sms)) return -1;
   if (!dense_path(c, a.heads, a.rows)) return attend_launch(a, ws, sms, d_status, st);
-  if (dense_rows(c) > 0x7fffffffll) return -1;
   uint16_t* k = static_cast<uint16_t*>(ws);
   uint16_t* v = k + static_cast<size_t>(dense_rows(c)) * c.kv_heads * 128;
   const int r = dense_launch(c, a.f16, k, v, d_status, st);

@@ -359,7 +359,8 @@ int exn_attn_cache_read(exn_attn* a, const exn_kv_cache* cache, int type, const 
  * ROWS (or more) and heads, 256-byte aligned, not shared by calls that may run at once; what it holds before and
  * after a call does not matter.  With few rows (tokens times query heads of a key/value head: up to 64 a
  * sequence on average and 64 more) the codes are read as they are; with more, they are turned into 16 bits
- * in the workspace once (4 * nseq * table_ld * 64 * kv_heads * 128 bytes).  Where lens[s] is less than
+ * in the workspace once (4 * nseq * table_ld * 64 * kv_heads * 128 bytes), unless nseq * table_ld is 2^25 or
+ * more, or 2^30 / kv_heads.  Where lens[s] is less than
  * the sequence's rows, the first rows see nothing and are 0. */
 int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int heads, const int32_t* offsets,
                           int64_t rows, const void* q, int64_t ld_q, void* out, int64_t ld_out, double scale,

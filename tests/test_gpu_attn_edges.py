@@ -336,3 +336,28 @@ def test_the_largest_numbers_stay_finite(att, t):
     many = torch.zeros(129, 1 * D, dtype=TYPES[t], device="cuda")
     out = c.attend(att, [129], many, 1, t)
     assert c.dense and torch.equal(out[-1], k[0])
+
+
+# --------------------------------------------------------------------------- tables with room for very many positions
+
+
+def test_chunks_over_tables_with_room_for_2_31_positions(att):
+    """More positions than one launch turns into 16 bits: the codes are read, with as little workspace."""
+    heads, kv_heads, lens, counts = 4, 1, [200, 70], [60, 70]
+    c = Cache(2, 4, kv_heads)
+    c.write(att, lens, rows(270, kv_heads, 1, "bf16"), rows(270, kv_heads, 2, "bf16"), "bf16")
+    few = att.cache_workspace(c.c, 1, heads)
+    ld = 2 ** 24 + 1
+    table = torch.full((2, ld), -1, dtype=torch.int32, device="cuda")
+    table[:, :4] = c.table
+    c.c.table, c.c.table_ld = table.data_ptr(), ld
+    q = rows(130, heads, 3, "bf16")
+    assert att.cache_workspace(c.c, 130, heads) == few
+    out = torch.full_like(q, 7.0)
+    space = torch.empty(few, dtype=torch.uint8, device="cuda")
+    o = offsets(counts)
+    att.cache_attend(c.c, q.data_ptr(), out.data_ptr(), o.data_ptr(), 130, heads, workspace=space.data_ptr(),
+                     workspace_bytes=few)
+    att.sync()
+    c.dense = False
+    c.check_attend(out, counts, q, heads, "bf16")
