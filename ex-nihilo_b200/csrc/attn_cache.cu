@@ -299,6 +299,9 @@ __global__ void __launch_bounds__(128) k_cache_read(const CacheArgs c, const int
 //     between 1 and 2^14 for it, so what fp16 drops (P' < 2^-25) is 2^-25 of the row's largest product of a
 //     weight and a scale, whatever the scales of the pages are.  The sums are rescaled only when the row
 //     maximum grows by more than 2^8 or P' would leave that range;
+//     The tensor core cuts its sums where other units round, so a warp's over n half pages come out low by
+//     about n 2^-24 of themselves (2^20 half pages over five warps: 1.1 %): 2^-11 and more only from 2^13 a warp on,
+//     which is a call over 100 GB of codes;
 //   * P^T turns from the first product's layout to the second's with movmatrix.
 constexpr int SPAN = 32;                  // positions a warp takes at a time
 constexpr int SPAN_BYTES = SPAN * 128;
@@ -520,7 +523,7 @@ __device__ __forceinline__ void attend_produce(const CUtensorMap* tmK, const CUt
   // Equal parts of the work end to end, of at least MIN_PART; or, when the items are so few that each can have
   // CTAs of its own and the longest one's parts are no longer for it, whole CTAs an item (a span a warp at
   // least): no CTA then takes more than one item.
-  int part_len = max(MIN_PART, (all_work + plan.ctas - 1) / plan.ctas);
+  int part_len = max(MIN_PART, all_work / plan.ctas + (all_work % plan.ctas ? 1 : 0));  // ALL_WORK: up to 2^31 - 1
   int stride = 0;  // an item's length when it has CTAs of its own: so many times part_len
   if (all_items > 0 && all_items <= plan.ctas) {
     const int each = min(plan.ctas / all_items, (longest + WARPS - 1) / WARPS);
@@ -536,7 +539,7 @@ __device__ __forceinline__ void attend_produce(const CUtensorMap* tmK, const CUt
   const int total = stride ? all_items * stride : all_work;  // below 2^31: stride < longest + ctas, items <= ctas
   work_here = work_here && f64 < total;
   int f = work_here ? static_cast<int>(f64) : 0;
-  const int fend = work_here ? min(f + part_len, total) : 0;
+  const int fend = work_here ? f + min(part_len, total - f) : 0;
   int seq = s_lo, count = end - start;
   int base = stride ? (items_to - items) * stride : work_to - work;
   if (work_here) {

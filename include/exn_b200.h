@@ -361,7 +361,8 @@ int exn_attn_cache_read(exn_attn* a, const exn_kv_cache* cache, int type, const 
  * sequence on average and 64 more) the codes are read as they are; with more, they are turned into 16 bits
  * in the workspace once (4 * nseq * table_ld * 64 * kv_heads * 128 bytes), unless nseq * table_ld is 2^25 or
  * more, or 2^30 / kv_heads.  Where lens[s] is less than
- * the sequence's rows, the first rows see nothing and are 0. */
+ * the sequence's rows, the first rows see nothing and are 0.  A 32nd of the sequences, one after another, may
+ * have less than 2^26 half pages to read over their heads and tiles of rows; more is reported as bad lengths. */
 int exn_attn_cache_attend(exn_attn* a, const exn_kv_cache* cache, int type, int heads, const int32_t* offsets,
                           int64_t rows, const void* q, int64_t ld_q, void* out, int64_t ld_out, double scale,
                           void* workspace, size_t workspace_bytes, void* stream);

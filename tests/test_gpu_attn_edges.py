@@ -361,3 +361,33 @@ def test_chunks_over_tables_with_room_for_2_31_positions(att):
     att.sync()
     c.dense = False
     c.check_attend(out, counts, q, heads, "bf16")
+
+
+def test_work_next_to_2_31(att):
+    """As much work as one call may have (2^26 half pages a run of the sequences, 2^31 in all): every sequence
+    is the same page again and again, so its rows are those over the page alone.
+
+    A warp adds up a fifth of an item, 2^20 / 5 half pages, in two products each, and the tensor core cuts what
+    is behind the last bit of a sum, up to 2^-23 of it, where other units round: 2 * 2^20 / 5 * 2^-23 = 5 % of A
+    at most, beside the usual bound."""
+    heads = kv_heads = 64
+    c = Cache(1, 1, kv_heads)
+    c.write(att, [64], rows(64, kv_heads, 1, "bf16"), rows(64, kv_heads, 2, "bf16"), "bf16")
+    q = rows(1, heads, 3, "bf16")
+    want = c.attend(att, [1], q, heads, "bf16")
+    c.check_attend(want, [1], q, heads, "bf16")
+    nseq, pages = 32, 2 ** 19 - 7  # 64 items of 2^20 - 14 + 12 a sequence
+    table = c.table[0, 0].repeat(nseq, pages)
+    lens = torch.full((nseq,), 64 * pages, dtype=torch.int32, device="cuda")
+    c.c.nseq, c.c.table_ld, c.c.table, c.c.lens = nseq, pages, table.data_ptr(), lens.data_ptr()
+    out = torch.full((nseq, heads * D), 7.0, dtype=torch.bfloat16, device="cuda")
+    o = offsets([1] * nseq)
+    qs = q.repeat(nseq, 1)
+    space = torch.empty(att.cache_workspace(c.c, nseq, heads), dtype=torch.uint8, device="cuda")
+    att.cache_attend(c.c, qs.data_ptr(), out.data_ptr(), o.data_ptr(), nseq, heads, workspace=space.data_ptr(),
+                     workspace_bytes=space.numel())
+    att.sync()
+    ref, a, absv = reference(q, c.model[0]["k"].cuda().flatten(1), c.model[0]["v"].cuda().flatten(1), heads, kv_heads)
+    tol = 2 ** -8 * ref.abs() + (2 ** -11 + 2 ** -11.5 + 0.05) * a + 2.0 ** -25 * (1 + absv)
+    worst = ((out.double() - ref).abs() / tol).max().item()
+    assert worst <= 1, "an output is %.3g of its bound off" % worst
