@@ -391,3 +391,73 @@ def test_work_next_to_2_31(att):
     tol = 2 ** -8 * ref.abs() + (2 ** -11 + 2 ** -11.5 + 0.05) * a + 2.0 ** -25 * (1 + absv)
     worst = ((out.double() - ref).abs() / tol).max().item()
     assert worst <= 1, "an output is %.3g of its bound off" % worst
+
+
+# --------------------------------------------------------------------------- what is not finite in a cache or beside one
+
+
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("name", ["k", "v"])
+@pytest.mark.parametrize("copies,tokens", [(1, 3), (400, 3), (1, 200)])
+def test_a_page_of_nan_reaches_the_rows_that_see_it(att, t, name, copies, tokens):
+    """A page whose keys or values were given a NaN after the first rows' positions, with a page of other
+    sizes before it: rows before its first position are right, the others NaN in its head, right in the next."""
+    heads, kv_heads, n = 4, 2, 64 * 6 + 1
+    c = Cache(1, 7, kv_heads)
+    k, v = rows(n, kv_heads, 1, t), rows(n, kv_heads, 2, t)
+    v[:128] *= 2.0 ** -6
+    c.write(att, [n], k, v, t)
+    page = c.table[0, 6].item()  # of the last position alone
+    c.scales[name][page, 0] = math.nan
+    q = rows(tokens, heads, 3, t)
+    if tokens > 64:
+        out = c.attend(att, [tokens], q, heads, t).reshape(1, tokens, -1)
+        assert c.dense
+    else:
+        out = attend_copies(att, c, q, heads, t, copies)
+    half = heads // 2 * D
+    assert torch.isnan(out[:, -1, :half]).all() and torch.isfinite(out[:, :-1]).all() and torch.isfinite(out[:, -1, half:]).all()
+    c.model[0] = {x: y[:-1] for x, y in c.model[0].items()}
+    c.scales[name][page, 0] = 1.0
+    c.lens.fill_(n - 1)
+    ref = reference(q[:-1], c.model[0]["k"].cuda().flatten(1), c.model[0]["v"].cuda().flatten(1), heads, kv_heads)
+    for x in out:
+        check(x[:-1], ref, t, p16="same" if tokens > 64 else "fp16")
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("tokens", [1, 3, 80])
+def test_a_query_that_is_not_finite_over_a_cache(att, value, tokens):
+    """It stays in its own output row and head, by either path."""
+    heads, kv_heads = 8, 2
+    c = Cache(2, 9, kv_heads)
+    lens = [500, 130]
+    c.write(att, lens, rows(630, kv_heads, 1, "bf16"), rows(630, kv_heads, 2, "bf16"), "bf16")
+    q = rows(2 * tokens, heads, 3, "bf16")
+    good = c.attend(att, [tokens] * 2, q, heads, "bf16")
+    assert c.dense == (tokens == 80)
+    for row, head in ((0, 1), (tokens, 6), (2 * tokens - 1, 0)):
+        bad = q.clone()
+        bad[row, head * D + 9] = value
+        out = c.attend(att, [tokens] * 2, bad, heads, "bf16")
+        touched = torch.zeros_like(good, dtype=torch.bool)
+        touched[row, head * D:(head + 1) * D] = True
+        assert torch.equal(out[~touched], good[~touched])
+        assert value == value or torch.isnan(out[touched]).all()
+
+
+def test_rows_without_any_sequence(att):
+    """Rows of which the offsets give none away: every call leaves its outputs as they are."""
+    c = Cache(3, 2, 2)
+    c.write(att, [70, 1, 0], rows(71, 2, 1, "bf16"), rows(71, 2, 2, "bf16"), "bf16")
+    before = [c.codes[x].clone() for x in "kv"]
+    x = rows(300, 8, 3, "bf16")
+    for n in (5, 300):
+        out = torch.full((n, 8 * D), 7.0, dtype=torch.bfloat16, device="cuda")
+        assert (c.attend(att, [0, 0, 0], x[:n], 8, "bf16", out=out) == 7).all()
+        assert (run_packed(att, x[:n], x[:n, :2 * D], x[:n, :2 * D], [0, 0], 8, 2, "bf16", out=out) == 7).all()
+        o = offsets([0, 0, 0])
+        att.cache_write(c.c, x.data_ptr(), x.data_ptr(), o.data_ptr(), n)
+        att.cache_read(c.c, out.data_ptr(), out.data_ptr(), o.data_ptr(), n)
+        att.sync()
+        assert (out == 7).all() and all(torch.equal(c.codes[y], z) for y, z in zip("kv", before))
