@@ -861,8 +861,7 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
         lim[nt][j] = row < nrows ? pos0 + row / nh : -1;
       }
 
-    // a row's maximum and sum of weights; log2 of its largest P 2^ev so far over 2^m (top) and of its sums' unit
-    // (unit, an integer)
+    // a row's maximum and sum of weights; log2 of its sums' unit (a whole number) and of its largest P' so far (top)
     float m[NT][2], l[NT][2], top[NT][2], unit[NT][2], o[NT][8][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -920,7 +919,7 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
       float s[NT][2][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float grown[2];  // how far the maximum grows
+        float most[2];  // the span's largest scores
         bool need = false;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -938,22 +937,29 @@ __global__ void __launch_bounds__(AttendCfg<NT>::THREADS, AttendCfg<NT>::CTAS)
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const bool grow = mx > m[nt][j] + 8.f;
-          grown[j] = grow ? mx - m[nt][j] : 0.f;
-          m[nt][j] = grow ? mx : m[nt][j];
-          const float mu = m[nt][j] == -INFINITY ? 0.f : m[nt][j];  // nothing seen yet: every P is 2^-inf = 0
-          top[nt][j] = fmaxf(top[nt][j] - grown[j], mx - mu + ev);
-          const float above = top[nt][j] - unit[nt][j];
-          need |= grow || above > 14.f || (above < 0.f && top[nt][j] > -INFINITY);
+          most[j] = mx;
+          const float d = mx - m[nt][j];  // infinite where the row sees its first position, NaN where it has seen none
+          top[nt][j] = fmaxf(top[nt][j], d + (ev - unit[nt][j]));
+          need |= d > 8.f || top[nt][j] > 14.f;
         }
         if (__any_sync(0xffffffffu, need)) {
           float f[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float above = top[nt][j] - unit[nt][j], before = unit[nt][j];
-            if (above > 14.f || (above < 0.f && top[nt][j] > -INFINITY)) unit[nt][j] = fminf(floorf(top[nt][j]), 127.f);
-            f[j] = fast_exp2(before - unit[nt][j] - grown[j]);  // at most 2: TOP fell by no more than the maximum grew
-            l[nt][j] *= fast_exp2(-grown[j]);
+            float grown = most[j] - m[nt][j], w = 0.f;
+            if (grown > 8.f) {
+              m[nt][j] = most[j];
+              top[nt][j] = grown < INFINITY ? top[nt][j] - grown : ev - unit[nt][j];
+            } else {
+              grown = 0.f;
+            }
+            if (top[nt][j] > 14.f || (top[nt][j] < 0.f && m[nt][j] > -INFINITY)) {
+              w = fminf(floorf(top[nt][j]), 127.f - unit[nt][j]);
+              unit[nt][j] += w;
+              top[nt][j] -= w;
+            }
+            f[j] = fast_exp2(-grown - w);  // at most 2: TOP falls by no more than the maximum grows
+            l[nt][j] *= fast_exp2(-grown);
           }
 #pragma unroll
           for (int q = 0; q < 8; ++q)
