@@ -100,8 +100,8 @@ __device__ __forceinline__ void find_page(const int* offsets, const int* lens, i
 }
 
 // ---- write: one block = one page touched by the call's rows, one key/value head, K or V; 16 threads a row of
-// 128 values.  Long prompts are bound by the bytes, 2 in and 1 out a value (6360 rows of 8 heads: 7.9 us, 5.0
-// TB/s); single tokens (64: 4.5 us) by the chain of dependent loads (offsets and lengths; the rows and the
+// 128 values.  Long prompts are bound by the bytes, 2 in and 1 out a value (6360 rows of 8 heads: 7.6 us, 5.1
+// TB/s); single tokens (64: 4.6 us) by the chain of dependent loads (offsets and lengths; the rows and the
 // table's entry; the page's scale; its codes, when the scale grows).
 template <bool F16>
 __global__ void __launch_bounds__(128) k_cache_write(const CacheArgs c, const int* __restrict__ offsets,
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(128) k_cache_write(const CacheArgs c, const in
 
 // ---- read: the same blocks; code * scale in 16 bits (exact in bf16; rounded once where fp16's range
 // ends).  DENSE: every position, to row s * table_ld * 64 + position.  Bound by the bytes, 1 in, 2 out
-// (7417 rows of 8 heads: 6.9 us, 6.6 TB/s).
+// (7157 rows of 8 heads: 7.0 us, 6.3 TB/s).
 template <bool F16, bool DENSE>
 __global__ void __launch_bounds__(128) k_cache_read(const CacheArgs c, const int* __restrict__ offsets,
                                                     long long rows, uint16_t* __restrict__ k, long long ld_k,
@@ -280,8 +280,8 @@ __global__ void __launch_bounds__(128) k_cache_read(const CacheArgs c, const int
 // is not taken for one.
 //
 // Bound by the codes' bytes (a code takes part in 4 g c operations) as long as the instructions keep up: 64
-// tokens over 500 to 8192 positions each, 335 MB, take 66.8 us (5.0 TB/s; 6.2 from the first copy to the last), one
-// over 130001, 266 MB, 54 us.  One over 1001 takes 9.7 us, all latency: launch 1.4, lengths and cut 1.8, the
+// tokens over 500 to 8192 positions each, 334 MB, take 66.5 us (5.0 TB/s; 6.2 from the first copy to the last), one
+// over 130001, 266 MB, 56 us.  One over 1001 takes 9.1 us, all latency: launch 1.4, lengths and cut 1.8, the
 // first span 2.7, the join over memory 3.
 // A byte permute, a logical operation and a paired fp16 one each take a scheduler two clocks a warp, an
 // MMA eight, so what turns codes into operands is what counts:
@@ -308,8 +308,8 @@ constexpr int SPAN_BYTES = SPAN * 128;
 constexpr int SETUP = 12;                 // what an item costs besides its spans, in spans
 constexpr int MIN_PART = 16 + SETUP;      // the least work worth a CTA that may take several items
 
-// Tiles of 8 rows (NT 1): two CTAs of 5 + 1 warps an SM, 168 registers a thread; of 16 rows, whose sums take
-// twice the registers, one of 7 + 1
+// Tiles of 8 rows (NT 1): two CTAs of 5 + 1 warps an SM, 168 registers a thread (20 bytes spilled); of 16 rows,
+// whose sums take twice the registers, one of 7 + 1, 255 (32 bytes)
 template <int NT>
 struct AttendCfg {
   static constexpr int WARPS = NT == 1 ? 5 : 7, CTAS = NT == 1 ? 2 : 1, ROWS = 8 * NT, THREADS = (WARPS + 1) * 32;
